@@ -25,6 +25,11 @@ OFFLOAD_ARCH = os.environ.get("FI_OFFLOAD_ARCH", "gfx950")
 
 HIPCC = os.environ.get("HIPCC", "hipcc")
 
+# No packed FP32 arithmetic (v_pk_{add,mul,fma}_f32): the compiler forms it
+# from ordinary float code, and some of its forms have given wrong results on
+# gfx950 now and then. hipcc's host pass does not know the feature and says so.
+NO_PACKED_FP32 = "-Xclang -target-feature -Xclang -packed-fp32-ops"
+
 
 def _torch_paths():
     import torch
@@ -38,7 +43,7 @@ def _gen_ninja() -> str:
     pyinc = sysconfig.get_paths()["include"]
     common = (
         f"-O3 -std=c++17 -fPIC --offload-arch={OFFLOAD_ARCH} "
-        f"-I{CSRC}/include -DNDEBUG"
+        f"-I{CSRC}/include -DNDEBUG {NO_PACKED_FP32}"
     )
     # Kernel TUs never see torch headers; binding TU does.
     bind_flags = (

@@ -201,7 +201,7 @@ __global__ __launch_bounds__(NTH, 2) void gemm_fp8_kernel(
     if constexpr (MODE == 1) {
       float sb = b_scales[((int64_t)seg * nk + kt) * ((N + 127) / 128) + bn0 / 128];
       float sab = ascale_s[cur][wm + line] * sb;
-      // packed f32 FMA halves the rescale VALU chain (v_pk_fma_f32)
+      // pairwise form; compiled without packed f32 math (see _build.py)
       typedef __attribute__((ext_vector_type(2))) float f32x2;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {

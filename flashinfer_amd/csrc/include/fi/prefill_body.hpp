@@ -420,8 +420,8 @@ __device__ __forceinline__ void prefill_tile_body(const PrefillParams& p, int re
       }
 
       // ---- online softmax update (per lane; exchange with lane^32).
-      // packed-f32 max/sum trees (v_pk_max/add_f32) halve the reduction
-      // VALU (PMC r02: VALUBusy 47% — the softmax chain IS the bound) ----
+      // pairwise max/sum trees; the library is compiled without packed f32
+      // math (see _build.py), so each pair is two scalar ops ----
       typedef __attribute__((ext_vector_type(2))) float f32x2_;
       const f32x2_* pr2 = reinterpret_cast<const f32x2_*>(pr);
       f32x2_ mx2 = pr2[0];

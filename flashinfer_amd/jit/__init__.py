@@ -20,6 +20,8 @@ from dataclasses import dataclass, field
 from pathlib import Path
 from typing import Dict, List, Optional, Sequence
 
+from .._build import NO_PACKED_FP32
+
 PKG_DIR = Path(__file__).resolve().parent.parent
 FI_INCLUDE = PKG_DIR / "csrc" / "include"
 
@@ -70,6 +72,7 @@ class JitSpec:
             h.update(self.sources[fn].encode())
         h.update(" ".join(self.extra_cflags + self.extra_ldflags).encode())
         h.update(self.offload_arch.encode())
+        h.update(NO_PACKED_FP32.encode())
         return h.hexdigest()[:16]
 
     @property
@@ -89,7 +92,7 @@ class JitSpec:
                 p.write_text(src)
         cflags = (
             f"-O3 -std=c++17 -fPIC --offload-arch={self.offload_arch} "
-            f"-I{FI_INCLUDE} " + " ".join(self.extra_cflags)
+            f"-I{FI_INCLUDE} {NO_PACKED_FP32} " + " ".join(self.extra_cflags)
         )
         lines = [
             "rule hip",
