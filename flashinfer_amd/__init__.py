@@ -55,9 +55,11 @@ from .fp8_quantization import (
     gemm_fp8_nt_groupwise,
     group_gemm_fp8_nt_groupwise,
     mm_fp8,
+    mxfp8_quantize,
     per_block_quant_fp8,
     per_token_group_quant_fp8,
 )
+from .mxfp4 import gemm_mxfp4_nt, gemm_mxfp4_nt_gated, mxfp4_quantize
 from . import comm
 from .parallel_attention import ParallelAttention, ring_attention
 from .decode import (
@@ -67,6 +69,7 @@ from .decode import (
 )
 from .norm import (
     fused_add_rmsnorm,
+    fused_add_rmsnorm_mxfp8_quant,
     fused_add_rmsnorm_quant,
     fused_rmsnorm_silu,
     fused_qk_rmsnorm_rope,
@@ -75,6 +78,7 @@ from .norm import (
     layernorm,
     layernorm_quant,
     rmsnorm,
+    rmsnorm_mxfp8_quant,
     rmsnorm_quant,
 )
 from .prefill import (

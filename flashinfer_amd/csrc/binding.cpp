@@ -89,6 +89,13 @@ hipError_t fi_gemm_fp8_grouped(const void* A, const void* W, void* C,
                                const float* a_scales, const float* b_scales,
                                float scalar_scale, int64_t a_scale_stride,
                                int flat_tiles, int mx, hipStream_t stream);
+hipError_t fi_mx_quant(int dtype, const void* x, void* residual, const void* w, void* out,
+                       void* scale, int rows, int k, int64_t sx, int64_t sr, float eps,
+                       int aligned, hipStream_t stream);
+hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act, const void* a,
+                         const void* a_scale, const void* b, const void* b_scale,
+                         void* out, void* out_scale, int M, int N, int K, int64_t lda,
+                         int64_t ldo, hipStream_t stream);
 hipError_t fi_per_group_quant_fp8(int dtype, int trans_scale, const void* x, void* q,
                                   float* scale, int64_t rows, int K, int64_t stride_row,
                                   float eps, hipStream_t stream);
@@ -893,6 +900,245 @@ void gemm_fp8_grouped(at::Tensor a, at::Tensor w, at::Tensor c, at::Tensor m_ind
             "fi_gemm_fp8_grouped");
 }
 
+// ---------------- MX formats ----------------
+
+// Whether two tensors of contiguous rows share memory. Rows at one distance
+// may lie beside each other, as column slices of one tensor do; rows at unlike
+// distances count as shared where the spans of the tensors meet.
+bool share_memory(const at::Tensor& x, const at::Tensor& y) {
+  if (x.numel() == 0 || y.numel() == 0) return false;
+  auto layout = [](const at::Tensor& t, uintptr_t& at, int64_t& width, int64_t& step) {
+    at = reinterpret_cast<uintptr_t>(t.data_ptr());
+    width = t.numel() * t.element_size();  // of one row, or of the whole
+    step = 0;
+    if (t.is_contiguous() && !(t.dim() == 2 && t.size(0) > 1)) return width;
+    width = t.size(-1) * t.element_size();
+    step = t.stride(0) * t.element_size();
+    return (t.size(0) - 1) * step + width;
+  };
+  uintptr_t a, b;
+  int64_t wa, wb, sa, sb;
+  const int64_t la = layout(x, a, wa, sa), lb = layout(y, b, wb, sb);
+  if (a + la <= b || b + lb <= a) return false;
+  if (sa != sb || sa == 0) return true;
+  const int64_t apart = (int64_t)((b - a) % (uintptr_t)sa);
+  const int64_t d = b >= a ? apart : (sa - (int64_t)((a - b) % (uintptr_t)sa)) % sa;
+  return d < wa || d + wb > sa;
+}
+
+void refuse_overlap(const char* name, const at::Tensor& out,
+                    std::initializer_list<const at::Tensor*> inputs) {
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK_VALUE(t == nullptr || !share_memory(out, *t), name,
+                      ": an output may not share memory with another operand");
+}
+
+bool is_scale(const at::Tensor& t) {
+  return t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat8_e8m0fnu;
+}
+
+bool on_16(const at::Tensor& t) {
+  return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+}
+
+// (out, out_scale) of x, of rmsnorm(x) * w, or of rmsnorm(residual += x) * w.
+std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tensor> residual,
+                                            c10::optional<at::Tensor> w,
+                                            c10::optional<at::Tensor> out,
+                                            c10::optional<at::Tensor> out_scale,
+                                            double eps) {
+  const char* name = "MXFP8 output";
+  TORCH_CHECK_VALUE(x.dim() >= 1, name, ": the input needs a last dimension");
+  const int64_t K = x.size(-1);
+  TORCH_CHECK_VALUE(K > 0 && K % 32 == 0 && K <= 65536, name,
+                    ": the last dimension must be a multiple of 32 up to 65536, got ", K);
+  TORCH_CHECK_VALUE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf ||
+                        x.scalar_type() == at::kFloat,
+                    name, ": the input is bfloat16, float16 or float32, got ",
+                    x.scalar_type());
+  const int64_t rows = x.numel() / K;
+  TORCH_CHECK_VALUE(rows < (int64_t(1) << 31), name, ": too many rows: ", rows);
+  // rows of one stride: contiguous, or two-dimensional
+  auto row_stride = [&](const at::Tensor& t, const char* what) -> int64_t {
+    if (t.is_contiguous()) return K;
+    TORCH_CHECK_VALUE(t.dim() == 2 && t.stride(1) == 1 && (t.size(0) == 1 || t.stride(0) >= K),
+                      name, ": ", what, " must be contiguous, or two-dimensional with "
+                      "contiguous rows that do not overlap, got strides ", t.strides());
+    return t.stride(0);
+  };
+  const int64_t sx = row_stride(x, "the input");
+  int64_t sr = 0;
+  if (residual) {
+    TORCH_CHECK_VALUE(residual->sizes() == x.sizes() &&
+                          residual->scalar_type() == x.scalar_type(),
+                      name, ": the residual must have the input's shape and type, got ",
+                      residual->scalar_type(), " ", residual->sizes());
+    sr = row_stride(*residual, "the residual");
+  }
+  if (w)
+    TORCH_CHECK_VALUE(w->dim() == 1 && w->size(0) == K && w->stride(0) == 1 &&
+                          w->scalar_type() == x.scalar_type(),
+                      name, ": the weight must be contiguous [", K, "] of the input's type, got ",
+                      w->scalar_type(), " ", w->sizes());
+  auto scale_shape = x.sizes().vec();
+  scale_shape.back() = K / 32;
+  if (out)
+    TORCH_CHECK_VALUE(out->sizes() == x.sizes() &&
+                          out->scalar_type() == at::kFloat8_e4m3fn && out->is_contiguous(),
+                      name, ": out must be contiguous float8_e4m3fn of the input's shape, got ",
+                      out->scalar_type(), " ", out->sizes());
+  if (out_scale)
+    TORCH_CHECK_VALUE(out_scale->sizes() == scale_shape &&
+                          out_scale->scalar_type() == at::kByte && out_scale->is_contiguous(),
+                      name, ": out_scale must be contiguous uint8 ", scale_shape, ", got ",
+                      out_scale->scalar_type(), " ", out_scale->sizes());
+  TORCH_CHECK_VALUE(x.is_cuda(), name, ": the input must be on a GPU, got ", x.device());
+  for (const auto* t : {&residual, &w, &out, &out_scale})
+    TORCH_CHECK_VALUE(!t->has_value() || (*t)->device() == x.device(), name,
+                      ": operands are on ", x.device(), " and ", (*t)->device());
+  const at::Tensor* r = residual ? &*residual : nullptr;
+  const at::Tensor* wp = w ? &*w : nullptr;
+  if (r) refuse_overlap(name, *r, {&x, wp});
+  if (out) refuse_overlap(name, *out, {&x, r, wp});
+  if (out_scale) refuse_overlap(name, *out_scale, {&x, r, wp, out ? &*out : nullptr});
+
+  c10::DeviceGuard guard(x.device());
+  at::Tensor q = out ? *out : at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+  at::Tensor s = out_scale ? *out_scale : at::empty(scale_shape, x.options().dtype(at::kByte));
+  const int64_t step = 16 / x.element_size();
+  const bool aligned = on_16(x) && (rows <= 1 || sx % step == 0) &&
+                       (!r || (on_16(*r) && (rows <= 1 || sr % step == 0))) &&
+                       (!wp || on_16(*wp)) &&
+                       reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0;
+  check_hip(fi_mx_quant(dtype_code(x), x.data_ptr(), r ? r->data_ptr() : nullptr,
+                        wp ? wp->data_ptr() : nullptr, q.data_ptr(), s.data_ptr(), (int)rows,
+                        (int)K, sx, sr, (float)eps, aligned, cur_stream(x)),
+            "fi_mx_quant");
+  return {q, s};
+}
+
+int mx_type(at::ScalarType t) {
+  return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat8_e4m3fn ? 2 : -1;
+}
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> mxfp4_product(
+    const char* name, bool gated, int64_t act, const at::Tensor& a, const at::Tensor& b,
+    const at::Tensor& b_scale, const c10::optional<at::Tensor>& a_scale,
+    const c10::optional<at::Tensor>& out, const c10::optional<at::Tensor>& out_scale,
+    c10::optional<at::ScalarType> out_dtype) {
+  TORCH_CHECK_VALUE(a.dim() == 2 && b.dim() == 2 && b_scale.dim() == 2, name,
+                    ": a, b and b_scale are two-dimensional, got ", a.sizes(), ", ", b.sizes(),
+                    ", ", b_scale.sizes());
+  const int a_type = mx_type(a.scalar_type());
+  TORCH_CHECK_VALUE(a_type >= 0, name, ": a is bfloat16, float16 or float8_e4m3fn, got ",
+                    a.scalar_type());
+  const int64_t M = a.size(0), K = a.size(1), rows = b.size(0);
+  TORCH_CHECK_VALUE(K > 0 && K % 32 == 0, name, ": K must be a multiple of 32, got ", K);
+  TORCH_CHECK_VALUE(b.scalar_type() == at::kByte && b.size(1) == K / 2 && b.is_contiguous(),
+                    name, ": b must be contiguous uint8 [", gated ? "2N, " : "N, ", K / 2,
+                    "] for K = ", K, ", got ", b.scalar_type(), " ", b.sizes(),
+                    " with strides ", b.strides());
+  TORCH_CHECK_VALUE(!gated || rows % 2 == 0, name,
+                    ": b holds the gate rows and as many up rows, got ", rows, " rows");
+  TORCH_CHECK_VALUE(is_scale(b_scale) && b_scale.size(0) == rows && b_scale.size(1) == K / 32 &&
+                        b_scale.is_contiguous(),
+                    name, ": b_scale must be contiguous uint8 [", rows, ", ", K / 32, "], got ",
+                    b_scale.scalar_type(), " ", b_scale.sizes());
+  TORCH_CHECK_VALUE((a_type == 2) == a_scale.has_value(), name,
+                    ": a_scale belongs to a float8_e4m3fn a and to no other");
+  if (a_scale)
+    TORCH_CHECK_VALUE(is_scale(*a_scale) && a_scale->dim() == 2 && a_scale->size(0) == M &&
+                          a_scale->size(1) == K / 32 && a_scale->is_contiguous(),
+                      name, ": a_scale must be contiguous uint8 [", M, ", ", K / 32, "], got ",
+                      a_scale->scalar_type(), " ", a_scale->sizes());
+  const int64_t N = gated ? rows / 2 : rows;
+  TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && rows < (int64_t(1) << 31) &&
+                        K < (int64_t(1) << 31),
+                    name, ": a dimension passes 2^31");
+  TORCH_CHECK_VALUE(M == 0 || (a.stride(1) == 1 &&
+                               (M == 1 || (a.stride(0) >= K &&
+                                           a.stride(0) * a.element_size() % 16 == 0)) &&
+                               on_16(a)),
+                    name, ": the rows of a must be contiguous, not overlap and start at "
+                    "multiples of 16 bytes, got strides ", a.strides());
+  TORCH_CHECK_VALUE(on_16(b), name, ": b must start at a multiple of 16 bytes");
+  const at::ScalarType type =
+      out_dtype ? *out_dtype
+                : out ? out->scalar_type() : a_type == 2 ? at::kBFloat16 : a.scalar_type();
+  const int out_type = mx_type(type);
+  const bool quantize = out_type == 2;
+  TORCH_CHECK_VALUE(out_type >= 0 && (gated || !quantize), name, ": out is bfloat16, float16",
+                    gated ? " or float8_e4m3fn" : "", ", got ", type);
+  TORCH_CHECK_VALUE(!quantize || N % 32 == 0, name,
+                    ": an MXFP8 output needs N to be a multiple of 32, got ", N);
+  if (out) {
+    TORCH_CHECK_VALUE(out->dim() == 2 && out->size(0) == M && out->size(1) == N &&
+                          out->scalar_type() == type,
+                      name, ": out must be ", type, " [", M, ", ", N, "], got ",
+                      out->scalar_type(), " ", out->sizes());
+    TORCH_CHECK_VALUE(out->numel() == 0 || ((N == 1 || out->stride(1) == 1) &&
+                                            (M == 1 || out->stride(0) >= N)),
+                      name, ": the rows of out must be contiguous and not overlap, got strides ",
+                      out->strides());
+    TORCH_CHECK_VALUE(!quantize || out->numel() == 0 ||
+                          (reinterpret_cast<uintptr_t>(out->data_ptr()) % 8 == 0 &&
+                           (M == 1 || out->stride(0) % 8 == 0)),
+                      name, ": the rows of an MXFP8 out must start at multiples of 8 bytes");
+  }
+  TORCH_CHECK_VALUE(!out_scale || quantize, name,
+                    ": out_scale belongs to a float8_e4m3fn output");
+  if (out_scale)
+    TORCH_CHECK_VALUE(out_scale->dim() == 2 && out_scale->size(0) == M &&
+                          out_scale->size(1) == N / 32 &&
+                          out_scale->scalar_type() == at::kByte && out_scale->is_contiguous(),
+                      name, ": out_scale must be contiguous uint8 [", M, ", ", N / 32, "], got ",
+                      out_scale->scalar_type(), " ", out_scale->sizes());
+  TORCH_CHECK_VALUE(a.is_cuda(), name, ": a must be on a GPU, got ", a.device());
+  auto same = [&](const at::Tensor& t) {
+    TORCH_CHECK_VALUE(t.device() == a.device(), name, ": operands are on ", a.device(), " and ",
+                      t.device());
+  };
+  same(b);
+  same(b_scale);
+  const at::Tensor* as = a_scale ? &*a_scale : nullptr;
+  if (as) same(*as);
+  if (out) {
+    same(*out);
+    refuse_overlap(name, *out, {&a, &b, &b_scale, as});
+  }
+  if (out_scale) {
+    same(*out_scale);
+    refuse_overlap(name, *out_scale, {&a, &b, &b_scale, as, out ? &*out : nullptr});
+  }
+
+  c10::DeviceGuard guard(a.device());
+  at::Tensor o = out ? *out : at::empty({M, N}, a.options().dtype(type));
+  c10::optional<at::Tensor> s;
+  if (quantize)
+    s = out_scale ? *out_scale : at::empty({M, N / 32}, a.options().dtype(at::kByte));
+  check_hip(fi_gemm_mxfp4(a_type, out_type, gated, (int)act, a.data_ptr(),
+                          as ? as->data_ptr() : nullptr, b.data_ptr(), b_scale.data_ptr(),
+                          o.data_ptr(), s ? s->data_ptr() : nullptr, (int)M, (int)N, (int)K,
+                          M > 1 ? a.stride(0) : K, M > 1 ? o.stride(0) : N, cur_stream(a)),
+            "fi_gemm_mxfp4");
+  return {o, s};
+}
+
+at::Tensor gemm_mxfp4_nt(at::Tensor a, at::Tensor b, at::Tensor b_scale,
+                         c10::optional<at::Tensor> a_scale, c10::optional<at::Tensor> out,
+                         c10::optional<at::ScalarType> out_dtype) {
+  return std::get<0>(mxfp4_product("gemm_mxfp4_nt", false, 0, a, b, b_scale, a_scale, out,
+                                   c10::nullopt, out_dtype));
+}
+
+std::tuple<at::Tensor, c10::optional<at::Tensor>> gemm_mxfp4_nt_gated(
+    at::Tensor a, at::Tensor b, at::Tensor b_scale, c10::optional<at::Tensor> a_scale,
+    int64_t act, c10::optional<at::Tensor> out, c10::optional<at::Tensor> out_scale,
+    c10::optional<at::ScalarType> out_dtype) {
+  return mxfp4_product("gemm_mxfp4_nt_gated", true, act, a, b, b_scale, a_scale, out, out_scale,
+                       out_dtype);
+}
+
 // per-128-group fp8 quantization: returns (q uint8 [rows,K], scale f32)
 void per_group_quant_fp8(at::Tensor x, at::Tensor q, at::Tensor scale,
                          bool trans_scale, double eps) {
@@ -1252,6 +1498,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("chain_speculative", &chain_speculative_op);
   m.def("mla_run", &mla_run);
   m.def("group_gemm_nt", &group_gemm_nt);
+  m.def("mx_quant", &mx_quant);
+  m.def("gemm_mxfp4_nt", &gemm_mxfp4_nt);
+  m.def("gemm_mxfp4_nt_gated", &gemm_mxfp4_nt_gated);
   m.def("gemm_fp8_grouped", &gemm_fp8_grouped);
   m.def("per_group_quant_fp8", &per_group_quant_fp8);
   m.def("scale_quant_fp8", &scale_quant_fp8);

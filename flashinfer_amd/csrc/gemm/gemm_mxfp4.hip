@@ -1,0 +1,312 @@
+// Products with MXFP4 weights for gfx950, plain and gated:
+//   out = a @ dequant(b)^T
+//   out = act(a @ dequant(b_gate)^T) * (a @ dequant(b_up)^T)
+// a: bf16 or fp16 rows, or MXFP8 (e4m3 with a scale byte for 32 neighbours);
+// b: [rows, K/2] packed e2m1, b_scale [rows, K/32]; the gated form holds the
+// N gate rows first, then the N up rows.
+//
+// Operand map, in 16x16 tiles (weights are the rows, tokens the columns):
+// lane l holds weight row l & 15 and, with g = l >> 4, the 32 values of block
+// g of a chunk of 128 - one load of 16 bytes and one scale byte.
+//   MXFP8 a: one v_mfma_scale_f32_16x16x128_f8f6f4 takes both operands as they
+//     lie in memory. Its fp8 operand holds k = 16g..16g+15 in the first four
+//     registers and 64+16g.. in the last four, its fp4 operand k = 32g..32g+31,
+//     and lane group g supplies the scale of block g for either.
+//   16-bit a: the block becomes bf16 (two values an instruction, the scale
+//     applied by it, exact for every scale) and feeds four 16x16x32 products;
+//     product i takes k = 32g + 8i .. 32g + 8i + 7 from lane group g.
+//   fp16 a: the same in fp16 where every scale of the wave's chunk keeps the
+//     weights exact in fp16 (2^-23 .. 2^13); elsewhere a is split into two
+//     bf16 parts, high and low, which hold its 11 bits exactly.
+// The products' sums are held in 32 bits. Within one instruction the matrix
+// unit aligns 8-bit products to the largest of them, which costs about 1e-5 of
+// the result on normal data; an output in 16 bits rounds to 4e-3 or 5e-4.
+#include "fi/common.hpp"
+#include "fi/mfma.hpp"
+#include "fi/mx.hpp"
+
+namespace fi {
+namespace mx4 {
+
+struct Params {
+  const void* a;
+  const uint8_t* a_scale;
+  const uint8_t* b;
+  const uint8_t* b_scale;
+  void* out;
+  uint8_t* out_scale;
+  int M, N, K;
+  int64_t lda, ldo;
+  int act;
+};
+
+enum { kBf16 = 0, kFp16 = 1, kFp8 = 2 };  // types of a
+// out: kBf16, kFp16, kFp8 (with scales)
+
+typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
+typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
+
+template <int kAct>
+__device__ __forceinline__ float activate(float g) {
+  if constexpr (kAct == 0) {
+    return g / (1.f + __builtin_expf(-g));
+  } else if constexpr (kAct == 1) {
+    // erfc keeps the small negative tail that 1 + erf rounds away
+    return 0.5f * g * erfcf(g * -0.70710678118654752f);
+  } else {
+    // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u))
+    const float u = 0.79788456080286536f * (g + 0.044715f * g * g * g);
+    return g / (1.f + __builtin_expf(-2.f * u));
+  }
+}
+
+__device__ __forceinline__ float activate(int act, float g) {
+  return act == 0 ? activate<0>(g) : act == 1 ? activate<1>(g) : activate<2>(g);
+}
+
+__device__ __forceinline__ float scale_value(uint32_t byte) {
+  // the conversions read the exponent bits alone: 0 is 2^-127, 255 is NaN
+  return __uint_as_float(byte << 23);
+}
+
+// Eight weights of one dword as bf16 or fp16, scaled.
+__device__ __forceinline__ bf16x8_t widen_bf16(uint32_t q, float s) {
+  union { bf16x8_t v; bf16x2_t p[4]; } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 0);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 1);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 2);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(q, s, 3);
+  return u.v;
+}
+__device__ __forceinline__ f16x8_t widen_f16(uint32_t q, float s) {
+  union { f16x8_t v; f16x2_t p[4]; } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 0);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 1);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 2);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(q, s, 3);
+  return u.v;
+}
+
+// fp16 as the sum of two bf16: 8 bits, then the remaining 3.
+__device__ __forceinline__ void split_f16(uint4 x, bf16x8_t& hi, bf16x8_t& lo) {
+  union { uint4 q; _Float16 h[8]; } u;
+  u.q = x;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float f = (float)u.h[j];
+    const __bf16 h = (__bf16)f;
+    hi[j] = h;
+    // an infinity has no remainder: inf - inf would make it a NaN
+    const float rest = f - (float)h;
+    lo[j] = (__bf16)(abs_bits(f) < 0x7f800000u ? rest : 0.f);
+  }
+}
+
+__device__ __forceinline__ bool f16_exact(uint32_t byte) {
+  return byte >= 104u && byte <= 140u;
+}
+
+// WAVES waves share a tile of RT * 16 outputs by MT * 16 tokens and take the
+// chunks of K in turn; their sums are joined in a fixed order.
+template <int ACT, bool GATED, int OUT, int RT, int MT, int WAVES>
+__global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
+  constexpr int AT = GATED ? 2 * RT : RT;  // weight tiles
+  constexpr int LD = AT * 16 + 4;
+  __shared__ __attribute__((aligned(16))) float red[WAVES][MT * 16][LD];
+
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lr = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * RT * 16, m0 = blockIdx.y * MT * 16;
+  const int blocks = p.K / kMxBlock;
+
+  const uint8_t* brow[AT];
+  const uint8_t* srow[AT];
+#pragma unroll
+  for (int t = 0; t < AT; ++t) {
+    const int n = n0 + (t % RT) * 16 + lr;
+    const int64_t row = (n < p.N ? n : p.N - 1) + (t >= RT ? (int64_t)p.N : 0);
+    brow[t] = p.b + row * (p.K / 2);
+    srow[t] = p.b_scale + row * blocks;
+  }
+  int64_t arow[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) {
+    const int m = m0 + t * 16 + lr;
+    arow[t] = m < p.M ? m : p.M - 1;
+  }
+
+  floatx4 acc[AT][MT];
+#pragma unroll
+  for (int i = 0; i < AT; ++i)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  for (int c = wave * 4; c < blocks; c += WAVES * 4) {
+    const int kb = c + g;
+    const bool in = kb < blocks;
+    uint4 w[AT];
+    uint32_t ws[AT];
+#pragma unroll
+    for (int t = 0; t < AT; ++t) {
+      w[t] = in ? *reinterpret_cast<const uint4*>(brow[t] + (int64_t)kb * 16)
+                : make_uint4(0, 0, 0, 0);
+      ws[t] = in ? srow[t][kb] : 127u;
+    }
+    if constexpr (ACT == kFp8) {
+#pragma unroll
+      for (int j = 0; j < MT; ++j) {
+        const uint8_t* ap = (const uint8_t*)p.a + arow[j] * p.lda + c * 32 + g * 16;
+        union { intx8 v; uint4 q[2]; } u;
+        u.q[0] = c + (g >> 1) < blocks ? *reinterpret_cast<const uint4*>(ap)
+                                       : make_uint4(0, 0, 0, 0);
+        u.q[1] = c + 2 + (g >> 1) < blocks ? *reinterpret_cast<const uint4*>(ap + 64)
+                                           : make_uint4(0, 0, 0, 0);
+        const uint32_t as = in ? p.a_scale[arow[j] * blocks + kb] : 127u;
+#pragma unroll
+        for (int t = 0; t < AT; ++t) {
+          intx8 wv = {(int)w[t].x, (int)w[t].y, (int)w[t].z, (int)w[t].w, 0, 0, 0, 0};
+          acc[t][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+              wv, u.v, acc[t][j], 4, 0, 0, (int)ws[t], 0, (int)as);
+        }
+      }
+    } else {
+      bool narrow = ACT == kFp16;
+      if constexpr (ACT == kFp16) {
+        bool ok = true;
+#pragma unroll
+        for (int t = 0; t < AT; ++t) ok = ok && f16_exact(ws[t]);
+        narrow = __all(ok);
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint4 x[MT];
+#pragma unroll
+        for (int j = 0; j < MT; ++j) {
+          const uint16_t* ap = (const uint16_t*)p.a + arow[j] * p.lda + (int64_t)kb * 32 + i * 8;
+          x[j] = in ? *reinterpret_cast<const uint4*>(ap) : make_uint4(0, 0, 0, 0);
+        }
+        if (narrow) {
+#pragma unroll
+          for (int t = 0; t < AT; ++t) {
+            const uint32_t q = i == 0 ? w[t].x : i == 1 ? w[t].y : i == 2 ? w[t].z : w[t].w;
+            const f16x8_t wv = widen_f16(q, scale_value(ws[t]));
+#pragma unroll
+            for (int j = 0; j < MT; ++j)
+              acc[t][j] = mfma_16x16x32_f16(wv, __builtin_bit_cast(f16x8_t, x[j]), acc[t][j]);
+          }
+        } else {
+          bf16x8_t hi[MT], lo[MT];
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            if constexpr (ACT == kFp16) split_f16(x[j], hi[j], lo[j]);
+            else hi[j] = __builtin_bit_cast(bf16x8_t, x[j]);
+          }
+#pragma unroll
+          for (int t = 0; t < AT; ++t) {
+            const uint32_t q = i == 0 ? w[t].x : i == 1 ? w[t].y : i == 2 ? w[t].z : w[t].w;
+            const bf16x8_t wv = widen_bf16(q, scale_value(ws[t]));
+#pragma unroll
+            for (int j = 0; j < MT; ++j) {
+              acc[t][j] = mfma_16x16x32_bf16(wv, hi[j], acc[t][j]);
+              if constexpr (ACT == kFp16) acc[t][j] = mfma_16x16x32_bf16(wv, lo[j], acc[t][j]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  // every lane's sums are needed below, also where its column is no token
+#pragma unroll
+  for (int t = 0; t < AT; ++t)
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      *reinterpret_cast<floatx4*>(&red[wave][j * 16 + lr][t * 16 + g * 4]) = acc[t][j];
+  __syncthreads();
+
+  // eight neighbouring outputs of one token to a thread
+  constexpr int G8 = RT * 2;
+  for (int i = threadIdx.x; i < MT * 16 * G8; i += WAVES * 64) {
+    const int ml = i / G8, nl = (i % G8) * 8;
+    const int m = m0 + ml, n = n0 + nl;
+    float y[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      float s = 0.f;
+#pragma unroll
+      for (int wv = 0; wv < WAVES; ++wv) s += red[wv][ml][nl + j];
+      if constexpr (GATED) {
+        float u = 0.f;
+#pragma unroll
+        for (int wv = 0; wv < WAVES; ++wv) u += red[wv][ml][RT * 16 + nl + j];
+        s = activate(p.act, s) * u;
+      }
+      y[j] = s;
+    }
+    if constexpr (OUT == kFp8) {
+      // N is a multiple of 32 here and a quad holds one block
+      uint32_t most = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) most = abs_bits(y[j]) > most ? abs_bits(y[j]) : most;
+      most = quad_max(most);
+      const uint32_t byte = mxfp8_scale_byte(most);
+      if (m < p.M && n < p.N) {
+        *reinterpret_cast<uint2*>((uint8_t*)p.out + (int64_t)m * p.ldo + n) =
+            mxfp8_pack8(y, mx_inverse_scale(byte), byte == 255u);
+        if (nl % 32 == 0)
+          p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
+      }
+    } else if (m < p.M) {
+      using T = typename std::conditional<OUT == kBf16, bf16, fp16>::type;
+      T* o = (T*)p.out + (int64_t)m * p.ldo + n;
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (n + j < p.N) o[j] = from_f32<T>(y[j]);
+    }
+  }
+}
+
+template <int ACT, bool GATED, int OUT>
+hipError_t launch(const Params& p, hipStream_t stream) {
+  constexpr int RT = OUT == kFp8 ? 2 : 1, MT = 1, WAVES = 4;
+  dim3 grid(ceil_div(p.N, RT * 16), ceil_div(p.M, MT * 16));
+  hipLaunchKernelGGL((rows_kernel<ACT, GATED, OUT, RT, MT, WAVES>), grid, dim3(WAVES * 64), 0,
+                     stream, p);
+  return hipGetLastError();
+}
+
+template <int ACT>
+hipError_t dispatch(bool gated, int out_type, const Params& p, hipStream_t stream) {
+  switch (out_type) {
+    case kBf16: return gated ? launch<ACT, true, kBf16>(p, stream) : launch<ACT, false, kBf16>(p, stream);
+    case kFp16: return gated ? launch<ACT, true, kFp16>(p, stream) : launch<ACT, false, kFp16>(p, stream);
+    case kFp8: if (gated) return launch<ACT, true, kFp8>(p, stream);
+  }
+  return hipErrorInvalidValue;
+}
+
+}  // namespace mx4
+}  // namespace fi
+
+// a_type / out_type: 0 bf16, 1 fp16, 2 e4m3 with scale bytes (as an output of
+// the gated form alone, N a multiple of 32). N counts outputs; the gated form
+// reads 2 * N weight rows. act: 0 silu, 1 gelu, 2 gelu with tanh. K is a
+// multiple of 32; rows of a, b and out start at multiples of 16 bytes (out:
+// where it is e4m3).
+extern "C" hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act,
+                                    const void* a, const void* a_scale, const void* b,
+                                    const void* b_scale, void* out, void* out_scale, int M,
+                                    int N, int K, int64_t lda, int64_t ldo,
+                                    hipStream_t stream) {
+  if (M == 0 || N == 0) return hipSuccess;
+  if (K <= 0 || K % fi::kMxBlock != 0) return hipErrorInvalidValue;
+  if (out_type == fi::mx4::kFp8 && N % fi::kMxBlock != 0) return hipErrorInvalidValue;
+  fi::mx4::Params p{a, (const uint8_t*)a_scale, (const uint8_t*)b, (const uint8_t*)b_scale,
+                    out, (uint8_t*)out_scale, M, N, K, lda, ldo, act};
+  switch (a_type) {
+    case 0: return fi::mx4::dispatch<fi::mx4::kBf16>(gated, out_type, p, stream);
+    case 1: return fi::mx4::dispatch<fi::mx4::kFp16>(gated, out_type, p, stream);
+    case 2: return fi::mx4::dispatch<fi::mx4::kFp8>(gated, out_type, p, stream);
+  }
+  return hipErrorInvalidValue;
+}

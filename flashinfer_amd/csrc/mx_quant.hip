@@ -1,0 +1,166 @@
+// MXFP8 output: an activation, or its RMSNorm (with or without the residual's
+// addition), written as e4m3 values with one scale for 32 neighbours.
+//
+//   r = x (+ residual, which is stored back rounded to its type)
+//   y = r / sqrt(mean(r^2) + eps) * w          (y = r without a weight)
+//   2^e: the least with max|y_block| <= 448 * 2^e;   q = e4m3(y * 2^-e)
+//
+// One workgroup takes one row and keeps it in registers, eight values to a
+// lane, so every input is read once and every output written once. The four
+// lanes of a quad hold one block of 32: its maximum needs two register
+// exchanges and no shared memory.
+#include "fi/common.hpp"
+#include "fi/mx.hpp"
+#include "fi/vec.hpp"
+
+namespace fi {
+namespace mxq {
+
+template <typename T, bool kAligned>
+__device__ __forceinline__ void load8(float* v, const T* p) {
+  vec_t<T, 8> t;
+  if constexpr (kAligned) {
+    t.load(p);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) t.data[j] = p[j];
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = t.get(j);
+}
+
+// NV: groups of eight values a lane holds. kAligned: 16-byte rows.
+template <typename T, int NV, bool kNorm, bool kAdd, bool kAligned>
+__global__ __launch_bounds__(1024) void mx_quant_kernel(
+    const T* __restrict__ x, T* __restrict__ residual, const T* __restrict__ w,
+    uint8_t* __restrict__ out, uint8_t* __restrict__ scale, int k, int64_t stride_x,
+    int64_t stride_r, float eps) {
+  __shared__ float sums[16];
+  const int64_t row = blockIdx.x;
+  const T* xr = x + row * stride_x;
+  T* rr = kAdd ? residual + row * stride_r : nullptr;
+  float v[NV][8];
+  float ss = 0.f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (i * blockDim.x + threadIdx.x) * 8;
+    if (at < k) {
+      load8<T, kAligned>(v[i], xr + at);
+      if constexpr (kAdd) {
+        float r[8];
+        load8<T, kAligned>(r, rr + at);
+        vec_t<T, 8> t;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          t.set(j, v[i][j] + r[j]);
+          v[i][j] = t.get(j);  // the norm is that of the residual as it is stored
+        }
+        if constexpr (kAligned) {
+          t.store(rr + at);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j) rr[at + j] = t.data[j];
+        }
+      }
+      if constexpr (kNorm) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+      }
+    }
+  }
+  float rrms = 1.f;
+  if constexpr (kNorm) {
+    ss = wave_reduce_sum<kWaveSize>(ss);
+    const int waves = blockDim.x / kWaveSize;
+    if (threadIdx.x % kWaveSize == 0) sums[threadIdx.x / kWaveSize] = ss;
+    __syncthreads();
+    ss = 0.f;
+    for (int i = 0; i < waves; ++i) ss += sums[i];
+    rrms = (float)(1.0 / sqrt((double)ss / k + (double)eps));
+  }
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int at = (i * blockDim.x + threadIdx.x) * 8;
+    if (at < k) {  // k is a multiple of 32: a quad is inside or outside as one
+      uint32_t most = 0;
+      float wv[8];
+      if constexpr (kNorm) load8<T, kAligned>(wv, w + at);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if constexpr (kNorm) v[i][j] = v[i][j] * rrms * wv[j];
+        const uint32_t b = abs_bits(v[i][j]);
+        most = b > most ? b : most;
+      }
+      most = quad_max(most);
+      const uint32_t byte = mxfp8_scale_byte(most);
+      const uint2 q = mxfp8_pack8(v[i], mx_inverse_scale(byte), byte == 255u);
+      uint8_t* o = out + row * k + at;
+      if constexpr (kAligned) {
+        *reinterpret_cast<uint2*>(o) = q;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[j] = (uint8_t)(q.x >> (8 * j));
+          o[4 + j] = (uint8_t)(q.y >> (8 * j));
+        }
+      }
+      if (threadIdx.x % 4 == 0) scale[row * (k / kMxBlock) + at / kMxBlock] = (uint8_t)byte;
+    }
+  }
+}
+
+template <typename T, bool kNorm, bool kAdd, bool kAligned>
+hipError_t launch(const void* x, void* residual, const void* w, void* out, void* scale,
+                  int rows, int k, int64_t sx, int64_t sr, float eps, hipStream_t stream) {
+  const int groups = k / 8;
+  int nv = 1;
+  while (nv < 8 && ceil_div(groups, nv) > 1024) nv *= 2;
+  const int threads = ceil_div(ceil_div(groups, nv), kWaveSize) * kWaveSize;
+  if (threads > 1024) return hipErrorInvalidValue;
+#define FI_GO(NV)                                                                       \
+  hipLaunchKernelGGL((mx_quant_kernel<T, NV, kNorm, kAdd, kAligned>), dim3(rows),       \
+                     dim3(threads), 0, stream, (const T*)x, (T*)residual, (const T*)w,  \
+                     (uint8_t*)out, (uint8_t*)scale, k, sx, sr, eps)
+  switch (nv) {
+    case 1: FI_GO(1); break;
+    case 2: FI_GO(2); break;
+    case 4: FI_GO(4); break;
+    default: FI_GO(8); break;
+  }
+#undef FI_GO
+  return hipGetLastError();
+}
+
+template <typename T>
+hipError_t dispatch(const void* x, void* residual, const void* w, void* out, void* scale,
+                    int rows, int k, int64_t sx, int64_t sr, float eps, int aligned,
+                    hipStream_t stream) {
+#define FI_GO(NORM, ADD)                                                                  \
+  (aligned ? launch<T, NORM, ADD, true>(x, residual, w, out, scale, rows, k, sx, sr, eps, \
+                                        stream)                                           \
+           : launch<T, NORM, ADD, false>(x, residual, w, out, scale, rows, k, sx, sr,     \
+                                         eps, stream))
+  if (!w) return FI_GO(false, false);
+  return residual ? FI_GO(true, true) : FI_GO(true, false);
+#undef FI_GO
+}
+
+}  // namespace mxq
+}  // namespace fi
+
+// dtype: 0 bf16, 1 fp16, 2 fp32. Without `w` the activation itself is written;
+// with `residual` x is added to it in place first. k: a multiple of 32, at
+// most 65536. `aligned`: x, residual and w have rows of whole 16 bytes, and
+// out starts at a multiple of 8.
+extern "C" hipError_t fi_mx_quant(int dtype, const void* x, void* residual, const void* w,
+                                  void* out, void* scale, int rows, int k, int64_t sx,
+                                  int64_t sr, float eps, int aligned, hipStream_t stream) {
+  if (rows == 0) return hipSuccess;
+  if (k <= 0 || k % fi::kMxBlock != 0 || k > 65536) return hipErrorInvalidValue;
+  switch (dtype) {
+    case 0: return fi::mxq::dispatch<fi::bf16>(x, residual, w, out, scale, rows, k, sx, sr, eps, aligned, stream);
+    case 1: return fi::mxq::dispatch<fi::fp16>(x, residual, w, out, scale, rows, k, sx, sr, eps, aligned, stream);
+    case 2: return fi::mxq::dispatch<float>(x, residual, w, out, scale, rows, k, sx, sr, eps, aligned, stream);
+  }
+  return hipErrorInvalidValue;
+}

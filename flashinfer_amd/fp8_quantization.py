@@ -30,6 +30,20 @@ def per_token_group_quant_fp8(
     return q.view(_FP8), scale
 
 
+def mxfp8_quantize(
+    x: torch.Tensor, out: Optional[torch.Tensor] = None,
+    out_scale: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    r"""An activation ``[..., K]`` (bf16, fp16 or fp32, K a multiple of 32 up to
+    65536) as MXFP8: ``(out, out_scale)``, e4m3 values of ``x``'s shape and one
+    scale byte for 32 neighbours (``[..., K // 32]`` uint8, the exponent of two
+    biased by 127). The scale is the least power of two with which no value of
+    its block saturates; a block that holds a NaN or an infinity is NaN throughout
+    (scale 255). What :func:`flashinfer_amd.gemm_mxfp4_nt` takes as ``a`` and
+    ``a_scale``."""
+    return get_ext().mx_quant(x, None, None, out, out_scale, 0.0)
+
+
 def per_block_quant_mxfp8(
     w: torch.Tensor, block: int = 128
 ) -> Tuple[torch.Tensor, torch.Tensor]:

@@ -1,0 +1,102 @@
+"""Products with MXFP4 weights: 4-bit values with one power-of-two scale for
+32 neighbours, the block format that the CDNA4 matrix unit reads directly.
+
+A weight ``[N, K]`` is held as ``b`` ``[N, K // 2]`` uint8 (two e2m1 values in
+a byte, the even ``k`` in the low half) and ``b_scale`` ``[N, K // 32]`` uint8
+(the exponent of two, biased by 127; 255 is NaN). Activations are bf16 or fp16,
+or MXFP8 as :func:`flashinfer_amd.mxfp8_quantize`,
+:func:`flashinfer_amd.fused_add_rmsnorm_mxfp8_quant` and
+:func:`gemm_mxfp4_nt_gated` itself write them."""
+from __future__ import annotations
+
+from typing import Optional, Tuple, Union
+
+import torch
+
+from ._lib import get_ext
+from .api_logging import flashinfer_api
+from .fi_trace import fi_trace
+
+MX_BLOCK = 32
+_ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
+
+
+def mxfp4_quantize(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    r"""Weights ``[..., N, K]`` as MXFP4: ``(b [..., N, K // 2], b_scale [..., N,
+    K // 32])``, both uint8. The scale is the least power of two with which no
+    value of its block saturates; values round to the nearest, ties to the one
+    with an even code. A block that holds a NaN or an infinity becomes NaN (scale
+    255). Done once when weights are loaded."""
+    if w.dim() < 2 or w.shape[-1] == 0 or w.shape[-1] % MX_BLOCK:
+        raise ValueError(
+            f"mxfp4_quantize needs [..., N, K] with K a multiple of {MX_BLOCK}, "
+            f"got {tuple(w.shape)}"
+        )
+    if not w.dtype.is_floating_point:
+        raise ValueError(f"mxfp4_quantize needs a floating type, got {w.dtype}")
+    blocks = w.float().unflatten(-1, (-1, MX_BLOCK))
+    most = blocks.abs().amax(-1)
+    mantissa, exponent = torch.frexp(most)
+    # most = mantissa * 2^exponent with mantissa in [.5, 1), and 6 = .75 * 2^3
+    exponent = (exponent - 3 + (mantissa > 0.75)).clamp(-127, 127)
+    bad = ~torch.isfinite(most)
+    exponent = torch.where(bad | (most == 0), torch.zeros_like(exponent), exponent)
+    scaled = torch.ldexp(blocks, -exponent.unsqueeze(-1))
+    a = scaled.abs()
+    # codes 0..7 are 0, .5, 1, 1.5, 2, 3, 4, 6; the middle of two neighbours
+    # goes to the even code: up from an odd code, down from an even one
+    code = torch.zeros(a.shape, dtype=torch.uint8, device=a.device)
+    for edge, up in ((0.25, False), (0.75, True), (1.25, False), (1.75, True),
+                     (2.5, False), (3.5, True), (5.0, False)):
+        code += (a >= edge) if up else (a > edge)
+    code |= torch.signbit(scaled).to(torch.uint8) << 3
+    code = torch.where(bad.unsqueeze(-1), torch.zeros_like(code), code).flatten(-2)
+    scale = torch.where(bad, torch.full_like(exponent, 255), exponent + 127)
+    return code[..., 0::2] | (code[..., 1::2] << 4), scale.to(torch.uint8)
+
+
+@flashinfer_api
+@fi_trace
+def gemm_mxfp4_nt(
+    a: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+    a_scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+) -> torch.Tensor:
+    r"""``out = a @ dequant(b, b_scale)^T`` with MXFP4 weights ``b`` [N, K // 2].
+
+    ``a`` [M, K] is bf16 or fp16, or MXFP8 (float8_e4m3fn with ``a_scale``
+    [M, K // 32]); its rows may be strided. ``out`` [M, N] is bf16 or fp16: by
+    default the type of a 16-bit ``a``, and bf16 for MXFP8. K is a multiple of 32;
+    M and N are any. Sums are held in 32 bits and rounded once. Operands start at
+    multiples of 16 bytes, the rows of ``a`` too; an output shares no memory with
+    an input."""
+    return get_ext().gemm_mxfp4_nt(a, b, b_scale, a_scale, out, out_dtype)
+
+
+@flashinfer_api
+@fi_trace
+def gemm_mxfp4_nt_gated(
+    a: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+    a_scale: Optional[torch.Tensor] = None, activation: str = "silu",
+    out: Optional[torch.Tensor] = None, out_scale: Optional[torch.Tensor] = None,
+    out_dtype: Optional[torch.dtype] = None,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    r"""A gated feed-forward block's first half in one kernel:
+    ``out = act(a @ dequant(b[:N])^T) * (a @ dequant(b[N:])^T)``.
+
+    ``b`` [2N, K // 2] holds the gate rows first, then the up rows (the order of
+    :func:`flashinfer_amd.silu_and_mul`); ``activation`` is ``"silu"``, ``"gelu"``
+    or ``"gelu_tanh"``. ``a`` as for :func:`gemm_mxfp4_nt`. With ``out_dtype``
+    (or an ``out``) of float8_e4m3fn the block is written as MXFP8 and
+    ``(out [M, N], out_scale [M, N // 32])`` is returned, as the next
+    :func:`gemm_mxfp4_nt` takes them; N is a multiple of 32 then. Neither
+    projection is rounded or written on the way."""
+    code = _ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(
+            f"gemm_mxfp4_nt_gated: activation is one of {sorted(_ACTIVATIONS)}, "
+            f"got {activation!r}"
+        )
+    out, out_scale = get_ext().gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, code, out,
+                                                   out_scale, out_dtype)
+    return out if out_scale is None else (out, out_scale)

@@ -3,7 +3,7 @@ from __future__ import annotations
 
 import functools
 
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -123,6 +123,42 @@ def fused_add_rmsnorm_quant(
     ``residual += input; out = (rmsnorm(residual) * weight / scale).to(fp8)``."""
     get_ext().rmsnorm_quant(_flat2d(input), _flat2d(residual), weight,
                             _flat2d(out), _scale_tensor(scale, input.device), eps)
+
+
+@flashinfer_api
+@fi_trace
+def rmsnorm_mxfp8_quant(
+    input: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    out: Optional[torch.Tensor] = None,
+    out_scale: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    r"""RMSNorm with an MXFP8 output: ``y = input / rms(input) * weight``, written
+    as ``(out, out_scale)``: e4m3 values of ``input``'s shape and one scale byte
+    for 32 neighbours (``[..., K // 32]`` uint8, the exponent of two biased by
+    127). The scale is the least power of two with which no value of its block
+    saturates; a block that holds a NaN or an infinity is NaN throughout (scale
+    255). ``input`` is bf16, fp16 or fp32 with K a multiple of 32 up to 65536; a
+    two-dimensional ``input`` may have strided rows. The scales come from the
+    32-bit norm itself, which is never rounded on the way."""
+    return get_ext().mx_quant(input, None, weight, out, out_scale, eps)
+
+
+@flashinfer_api
+@fi_trace
+def fused_add_rmsnorm_mxfp8_quant(
+    input: torch.Tensor,
+    residual: torch.Tensor,
+    weight: torch.Tensor,
+    eps: float = 1e-6,
+    out: Optional[torch.Tensor] = None,
+    out_scale: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    r"""In place ``residual += input``, then the RMSNorm of the residual as it is
+    stored, written as MXFP8: returns ``(out, out_scale)`` as
+    :func:`rmsnorm_mxfp8_quant` does."""
+    return get_ext().mx_quant(input, residual, weight, out, out_scale, eps)
 
 
 @flashinfer_api
