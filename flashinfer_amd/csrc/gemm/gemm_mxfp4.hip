@@ -266,8 +266,353 @@ __global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
   }
 }
 
+// ---------------------------------------------------------------------------
+// Many tokens: a workgroup of GN x GM waves computes a tile of GN * WN * 32
+// weight rows by GM * WM * 32 tokens in 32x32 products. Steps of 128 bytes of
+// a token row (128 values in 8 bits, 64 in 16) go to shared memory with their
+// weights, two buffers in turn, by loads that bypass the registers; the scales
+// of 512 values of a row come as 16 bytes once per 512.
+//
+// Operand map of 32x32: lane l holds row (token) l & 31 and, with g = l >> 5,
+//   8-bit a, 32x32x64: fp4 k = 32g..32g+31; fp8 k = 16g..16g+15 and 32+16g..;
+//     lane group g supplies the scale of block g.
+//   16-bit a, 32x32x16, product i of 4 in a step: k = 32g + 8i .. 32g + 8i + 7,
+//     so that a lane's weights are one block of one scale here as well.
+
+template <int WB>  // bytes of a row in the buffer: 16-byte units spread over the banks
+__device__ __forceinline__ uint32_t lds_at(int row, int byte) {
+  const uint32_t off = (uint32_t)(row * WB + byte);
+  return off ^ (((off >> 8) & 15) << 4);
+}
+
+template <int ACT, bool GATED, int WN, int WM, int GN, int GM>
+struct Tile {
+  static constexpr int kThreads = GN * GM * 64;
+  static constexpr int TN = GN * WN * 32, TM = GM * WM * 32;
+  static constexpr int kOut = GATED ? TN / 2 : TN;       // outputs of a tile along N
+  static constexpr int KS = ACT == kFp8 ? 128 : 64;      // values of a step
+  static constexpr int WB = KS / 2;                      // bytes of a weight row in a step
+  static constexpr int kSteps = 512 / KS;                // steps of one load of scales
+  static constexpr int kABytes = TM * 128, kBBytes = TN * WB;
+  static constexpr int kSRows = TN + (ACT == kFp8 ? TM : 0);
+  static constexpr int kLds = 2 * (kABytes + kBBytes) + 2 * 16 * kSRows;
+  static constexpr int AU = kABytes / 16 / kThreads, BU = kBBytes / 16 / kThreads;
+  static constexpr int SU = (kSRows + kThreads - 1) / kThreads;
+  static_assert(AU * 16 * kThreads == kABytes && BU * 16 * kThreads == kBBytes, "");
+};
+
+// the weight row (of N, or of 2N where gated) that row r of a tile stands for
+template <bool GATED, int WN>
+__device__ __forceinline__ int64_t weight_row(int n0, int r, int N) {
+  if constexpr (!GATED) {
+    const int n = n0 + r;
+    return n < N ? n : N - 1;
+  } else {
+    constexpr int H = WN / 2;  // a wave holds H tiles of gate rows, then H of up rows
+    const int wave = r / (WN * 32), t = r / 32 % WN;
+    const int n = n0 + (wave * H + t % H) * 32 + r % 32;
+    return (n < N ? n : N - 1) + (t >= H ? (int64_t)N : 0);
+  }
+}
+
+__device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t dst) {
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                   (__attribute__((address_space(3))) void*)(uintptr_t)dst, 16, 0,
+                                   0);
+}
+
+template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
+__global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_n, int tiles_m) {
+  using C = Tile<ACT, GATED, WN, WM, GN, GM>;
+  __shared__ __attribute__((aligned(256))) uint8_t lds[C::kLds];
+  uint8_t* const lds_a = lds;
+  uint8_t* const lds_b = lds + 2 * C::kABytes;
+  uint32_t* const lds_s = (uint32_t*)(lds + 2 * (C::kABytes + C::kBBytes));  // [2][4][kSRows]
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wn = wave % GN, wm = wave / GN;
+  const int lr = lane & 31, g = lane >> 5;
+
+  // neighbouring tiles run on one XCD, in bands of eight tiles of tokens
+  const int id = (int)xcd_swizzle(blockIdx.x, gridDim.x);
+  const int band = id / (8 * tiles_n), first = band * 8;
+  const int high = tiles_m - first < 8 ? tiles_m - first : 8;
+  const int in_band = id - band * 8 * tiles_n;
+  const int m0 = (first + in_band % high) * C::TM, n0 = in_band / high * C::kOut;
+
+  const int blocks = p.K / kMxBlock;
+  const int steps = (p.K + C::KS - 1) / C::KS;
+  const int64_t a_step = 128;
+  const int64_t a_row_bytes = p.lda * (ACT == kFp8 ? 1 : 2);
+
+  // where this thread's 16-byte units come from: dst is linear, src permuted
+  const uint8_t* a_src[C::AU];
+  const uint8_t* b_src[C::BU];
+#pragma unroll
+  for (int i = 0; i < C::AU; ++i) {
+    const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
+    const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+    const int m = m0 + (int)(off / 128);
+    a_src[i] = (const uint8_t*)p.a + (int64_t)(m < p.M ? m : p.M - 1) * a_row_bytes + off % 128;
+  }
+#pragma unroll
+  for (int i = 0; i < C::BU; ++i) {
+    const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
+    const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+    b_src[i] = p.b + weight_row<GATED, WN>(n0, (int)(off / C::WB), p.N) * (p.K / 2) + off % C::WB;
+  }
+  const uint32_t a_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_a;
+  const uint32_t b_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_b;
+
+  auto stage = [&](int t, int buf) {
+    if ((t + 1) * C::KS <= p.K) {
+#pragma unroll
+      for (int i = 0; i < C::AU; ++i)
+        load_lds16(a_src[i] + t * a_step,
+                   a_base + buf * C::kABytes + (uint32_t)(tid + i * C::kThreads) * 16);
+#pragma unroll
+      for (int i = 0; i < C::BU; ++i)
+        load_lds16(b_src[i] + (int64_t)t * C::WB,
+                   b_base + buf * C::kBBytes + (uint32_t)(tid + i * C::kThreads) * 16);
+    } else {
+      // the last step of a K that is no multiple of it: zeros behind the end
+      const int left = p.K - t * C::KS;  // values
+#pragma unroll
+      for (int i = 0; i < C::AU; ++i) {
+        const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
+        const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+        const bool in = (int)(off % 128) < left * (ACT == kFp8 ? 1 : 2);
+        *(uint4*)(lds_a + buf * C::kABytes + dst) =
+            in ? *(const uint4*)(a_src[i] + t * a_step) : make_uint4(0, 0, 0, 0);
+      }
+#pragma unroll
+      for (int i = 0; i < C::BU; ++i) {
+        const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
+        const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+        const bool in = (int)(off % C::WB) < left / 2;
+        *(uint4*)(lds_b + buf * C::kBBytes + dst) =
+            in ? *(const uint4*)(b_src[i] + (int64_t)t * C::WB) : make_uint4(0, 0, 0, 0);
+      }
+    }
+  };
+
+  // scales of blocks 16u .. 16u + 15 of every row of the tile
+  auto scales = [&](int u, uint32_t (&v)[C::SU][4]) {
+#pragma unroll
+    for (int i = 0; i < C::SU; ++i) {
+      const int r = tid + i * C::kThreads;
+      if (r >= C::kSRows) break;
+      const uint8_t* src;
+      if (r < C::TN) {
+        src = p.b_scale + weight_row<GATED, WN>(n0, r, p.N) * blocks;
+      } else {
+        const int m = m0 + r - C::TN;
+        src = p.a_scale + (int64_t)(m < p.M ? m : p.M - 1) * blocks;
+      }
+      if ((u + 1) * 16 <= blocks) {
+        __builtin_memcpy(v[i], src + u * 16, 16);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          v[i][j] = 0;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const int at = u * 16 + j * 4 + k;
+            v[i][j] |= (at < blocks ? (uint32_t)src[at] : 127u) << (8 * k);
+          }
+        }
+      }
+    }
+  };
+  auto put_scales = [&](int buf, const uint32_t (&v)[C::SU][4]) {
+#pragma unroll
+    for (int i = 0; i < C::SU; ++i) {
+      const int r = tid + i * C::kThreads;
+      if (r >= C::kSRows) break;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) lds_s[(buf * 4 + j) * C::kSRows + r] = v[i][j];
+    }
+  };
+
+  floatx16 acc[WN][WM];
+#pragma unroll
+  for (int i = 0; i < WN; ++i)
+#pragma unroll
+    for (int j = 0; j < WM; ++j) acc[i][j] = {};
+
+  uint32_t sv[C::SU][4];
+  scales(0, sv);
+  stage(0, 0);
+  put_scales(0, sv);
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+
+  const int b_row = wn * WN * 32 + lr, a_row = wm * WM * 32 + lr;
+  for (int t = 0; t < steps; ++t) {
+    const int buf = t & 1, u = t / C::kSteps, s = t % C::kSteps;
+    const bool more = (u + 1) * 16 < blocks;
+    if (t + 1 < steps) stage(t + 1, buf ^ 1);
+    if (s == 0 && more) scales(u + 1, sv);
+
+    const uint8_t* la = lds_a + buf * C::kABytes;
+    const uint8_t* lb = lds_b + buf * C::kBBytes;
+    const uint32_t* ls = lds_s + ((u & 1) * 4 + s * 4 / C::kSteps) * C::kSRows;
+    uint32_t ws[WN];
+#pragma unroll
+    for (int i = 0; i < WN; ++i) ws[i] = ls[b_row + i * 32] >> (8 * g);
+    if constexpr (ACT == kFp8) {
+      uint32_t as[WM];
+#pragma unroll
+      for (int j = 0; j < WM; ++j) as[j] = ls[C::TN + a_row + j * 32] >> (8 * g);
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        union { intx8 v; uint4 q[2]; } x[WM];
+        uint4 w[WN];
+#pragma unroll
+        for (int i = 0; i < WN; ++i)
+          w[i] = *(const uint4*)(lb + lds_at<C::WB>(b_row + i * 32, k * 32 + g * 16));
+#pragma unroll
+        for (int j = 0; j < WM; ++j) {
+          x[j].q[0] = *(const uint4*)(la + lds_at<128>(a_row + j * 32, k * 64 + g * 16));
+          x[j].q[1] = *(const uint4*)(la + lds_at<128>(a_row + j * 32, k * 64 + 32 + g * 16));
+        }
+#pragma unroll
+        for (int i = 0; i < WN; ++i) {
+          const intx8 wv = {(int)w[i].x, (int)w[i].y, (int)w[i].z, (int)w[i].w, 0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < WM; ++j) {
+            // bytes 2k and 2k + 1 of the step's scales belong to this product
+            if (k == 0)
+              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                  wv, x[j].v, acc[i][j], 4, 0, 0, (int)ws[i], 0, (int)as[j]);
+            else
+              acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+                  wv, x[j].v, acc[i][j], 4, 0, 2, (int)ws[i], 2, (int)as[j]);
+          }
+        }
+      }
+    } else {
+      uint4 w[WN];
+      bool narrow = ACT == kFp16;
+#pragma unroll
+      for (int i = 0; i < WN; ++i) {
+        w[i] = *(const uint4*)(lb + lds_at<C::WB>(b_row + i * 32, g * 16));
+        ws[i] = ws[i] >> (16 * (s & 1)) & 255u;  // two steps to a dword
+      }
+      if constexpr (ACT == kFp16) {
+        bool ok = true;
+#pragma unroll
+        for (int i = 0; i < WN; ++i) ok = ok && f16_exact(ws[i]);
+        narrow = __all(ok);
+      }
+      if (narrow || ACT == kBf16) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint4 x[WM];
+#pragma unroll
+          for (int j = 0; j < WM; ++j)
+            x[j] = *(const uint4*)(la + lds_at<128>(a_row + j * 32, g * 64 + k * 16));
+#pragma unroll
+          for (int i = 0; i < WN; ++i) {
+            const uint32_t q = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
+            if constexpr (ACT == kFp16) {
+              const f16x8_t wv = widen_f16(q, scale_value(ws[i]));
+#pragma unroll
+              for (int j = 0; j < WM; ++j)
+                acc[i][j] = mfma_32x32x16_f16(wv, __builtin_bit_cast(f16x8_t, x[j]), acc[i][j]);
+            } else {
+              const bf16x8_t wv = widen_bf16(q, scale_value(ws[i]));
+#pragma unroll
+              for (int j = 0; j < WM; ++j)
+                acc[i][j] = mfma_32x32x16_bf16(wv, __builtin_bit_cast(bf16x8_t, x[j]), acc[i][j]);
+            }
+          }
+        }
+      } else {
+        // rare: kept small rather than fast
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) {
+#pragma unroll
+          for (int j = 0; j < WM; ++j) {
+            const uint4 x = *(const uint4*)(la + lds_at<128>(a_row + j * 32, g * 64 + k * 16));
+            bf16x8_t hi, lo;
+            split_f16(x, hi, lo);
+#pragma unroll
+            for (int i = 0; i < WN; ++i) {
+              const uint32_t q = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
+              const bf16x8_t wv = widen_bf16(q, scale_value(ws[i]));
+              acc[i][j] = mfma_32x32x16_bf16(wv, hi, acc[i][j]);
+              acc[i][j] = mfma_32x32x16_bf16(wv, lo, acc[i][j]);
+            }
+          }
+        }
+      }
+    }
+    if (s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
+    // the buffers of the next step are full, and this step's are free
+    __builtin_amdgcn_s_waitcnt(0);
+    __syncthreads();
+  }
+
+  // lane: token lr of a tile; register r: output (r & 3) + 8 (r >> 2) + 4 g
+#pragma unroll
+  for (int j = 0; j < WM; ++j) {
+    const int m = m0 + a_row + j * 32;
+    constexpr int H = GATED ? WN / 2 : WN;
+#pragma unroll
+    for (int i = 0; i < H; ++i) {
+      const int n = n0 + (wn * H + i) * 32 + 4 * g;
+      float y[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        y[r] = GATED ? activate(p.act, acc[i][j][r]) * acc[i + (GATED ? H : 0)][j][r]
+                     : acc[i][j][r];
+      if constexpr (OUT == kFp8) {
+        uint32_t most = 0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) most = abs_bits(y[r]) > most ? abs_bits(y[r]) : most;
+        uint32_t a, b;
+        permlane32_pair(most, most, a, b);  // the other half of the block
+        most = a > b ? a : b;
+        const uint32_t byte = mxfp8_scale_byte(most);
+        const float inv = mx_inverse_scale(byte);
+        if (m < p.M && n - 4 * g < p.N) {
+          uint8_t* o = (uint8_t*)p.out + (int64_t)m * p.ldo + n;
+#pragma unroll
+          for (int r = 0; r < 16; r += 8) {
+            const uint2 q = mxfp8_pack8(y + r, inv, byte == 255u);
+            *(uint32_t*)(o + r * 2) = q.x;
+            *(uint32_t*)(o + r * 2 + 8) = q.y;
+          }
+          if (g == 0)
+            p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
+        }
+      } else if (m < p.M) {
+        using T = typename std::conditional<OUT == kBf16, bf16, fp16>::type;
+        T* o = (T*)p.out + (int64_t)m * p.ldo + n;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (n + (r & 3) + 8 * (r >> 2) < p.N) o[(r & 3) + 8 * (r >> 2)] = from_f32<T>(y[r]);
+      }
+    }
+  }
+}
+
+template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
+hipError_t launch_tile(const Params& p, hipStream_t stream) {
+  using C = Tile<ACT, GATED, WN, WM, GN, GM>;
+  const int64_t tiles_n = ceil_div(p.N, C::kOut), tiles_m = ceil_div(p.M, C::TM);
+  if (tiles_n * tiles_m >= (int64_t)1 << 31) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((tile_kernel<ACT, GATED, OUT, WN, WM, GN, GM>),
+                     dim3((unsigned)(tiles_n * tiles_m)), dim3(C::kThreads), 0, stream, p,
+                     (int)tiles_n, (int)tiles_m);
+  return hipGetLastError();
+}
+
 template <int ACT, bool GATED, int OUT>
 hipError_t launch(const Params& p, hipStream_t stream) {
+  if (p.M > 64) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 2>(p, stream);
   constexpr int RT = OUT == kFp8 ? 2 : 1, MT = 1, WAVES = 4;
   dim3 grid(ceil_div(p.N, RT * 16), ceil_div(p.M, MT * 16));
   hipLaunchKernelGGL((rows_kernel<ACT, GATED, OUT, RT, MT, WAVES>), grid, dim3(WAVES * 64), 0,
