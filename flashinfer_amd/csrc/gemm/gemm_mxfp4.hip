@@ -270,7 +270,7 @@ __global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
 // Many tokens: a workgroup of GN x GM waves computes a tile of GN * WN * 32
 // weight rows by GM * WM * 32 tokens in 32x32 products. Steps of 128 bytes of
 // a token row (128 values in 8 bits, 64 in 16) go to shared memory with their
-// weights, two buffers in turn, by loads that bypass the registers; the scales
+// weights, three buffers in turn, by loads that bypass the registers; the scales
 // of 512 values of a row come as 16 bytes once per 512.
 //
 // Operand map of 32x32: lane l holds row (token) l & 31 and, with g = l >> 5,
@@ -288,6 +288,7 @@ __device__ __forceinline__ uint32_t lds_at(int row, int byte) {
 template <int ACT, bool GATED, int WN, int WM, int GN, int GM>
 struct Tile {
   static constexpr int kThreads = GN * GM * 64;
+  static constexpr int kBufs = 3;
   static constexpr int TN = GN * WN * 32, TM = GM * WM * 32;
   static constexpr int kOut = GATED ? TN / 2 : TN;       // outputs of a tile along N
   static constexpr int KS = ACT == kFp8 ? 128 : 64;      // values of a step
@@ -295,30 +296,36 @@ struct Tile {
   static constexpr int kSteps = 512 / KS;                // steps of one load of scales
   static constexpr int kABytes = TM * 128, kBBytes = TN * WB;
   static constexpr int kSRows = TN + (ACT == kFp8 ? TM : 0);
-  static constexpr int kLds = 2 * (kABytes + kBBytes) + 2 * 16 * kSRows;
+  static constexpr int kLds = kBufs * (kABytes + kBBytes) + 2 * 16 * kSRows;
   static constexpr int AU = kABytes / 16 / kThreads, BU = kBBytes / 16 / kThreads;
+  static constexpr int kInFlight = AU + BU;              // loads a wave issues for a step
   static constexpr int SU = (kSRows + kThreads - 1) / kThreads;
   static_assert(AU * 16 * kThreads == kABytes && BU * 16 * kThreads == kBBytes, "");
 };
 
-// the weight row (of N, or of 2N where gated) that row r of a tile stands for
+// Row r of a tile of weights: a wave holds WN tiles of 32, where gated half of
+// them gate rows and half the up rows of the same outputs.
 template <bool GATED, int WN>
-__device__ __forceinline__ int64_t weight_row(int n0, int r, int N) {
-  if constexpr (!GATED) {
-    const int n = n0 + r;
-    return n < N ? n : N - 1;
-  } else {
-    constexpr int H = WN / 2;  // a wave holds H tiles of gate rows, then H of up rows
-    const int wave = r / (WN * 32), t = r / 32 % WN;
-    const int n = n0 + (wave * H + t % H) * 32 + r % 32;
-    return (n < N ? n : N - 1) + (t >= H ? (int64_t)N : 0);
-  }
+__device__ __forceinline__ bool is_up(int r) {
+  return GATED && r / 32 % WN >= WN / 2;
+}
+// its output, counted from n0 and held inside N
+template <bool GATED, int WN>
+__device__ __forceinline__ int weight_row(int n0, int r, int N) {
+  if constexpr (GATED) r = (r / (WN * 32) * (WN / 2) + r / 32 % (WN / 2)) * 32 + r % 32;
+  return n0 + r < N ? r : N - 1 - n0;
 }
 
-__device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t dst) {
-  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
-                                   (__attribute__((address_space(3))) void*)(uintptr_t)dst, 16, 0,
-                                   0);
+// 16 bytes a lane from base + at to the wave's 1024 at `dst` (a wave's own, uniform
+// address). In assembly, for the compiler holds every read of shared memory
+// behind such a load, also where the two go to different buffers: with the
+// builtin the next step's loads were waited for before this step's products.
+// Nothing waits for it here: s_waitcnt vmcnt before the barrier does.
+__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t at, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(dst), "v"(at), "s"(base)
+               : "memory");
 }
 
 template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
@@ -326,8 +333,8 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
   using C = Tile<ACT, GATED, WN, WM, GN, GM>;
   __shared__ __attribute__((aligned(256))) uint8_t lds[C::kLds];
   uint8_t* const lds_a = lds;
-  uint8_t* const lds_b = lds + 2 * C::kABytes;
-  uint32_t* const lds_s = (uint32_t*)(lds + 2 * (C::kABytes + C::kBBytes));  // [2][4][kSRows]
+  uint8_t* const lds_b = lds + C::kBufs * C::kABytes;
+  uint32_t* const lds_s = (uint32_t*)(lds + C::kBufs * (C::kABytes + C::kBBytes));  // [2][4][kSRows]
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -343,24 +350,30 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
 
   const int blocks = p.K / kMxBlock;
   const int steps = (p.K + C::KS - 1) / C::KS;
-  const int64_t a_step = 128;
   const int64_t a_row_bytes = p.lda * (ACT == kFp8 ? 1 : 2);
 
-  // where this thread's 16-byte units come from: dst is linear, src permuted
-  const uint8_t* a_src[C::AU];
-  const uint8_t* b_src[C::BU];
+  // where this thread's 16-byte units come from: dst is linear, src permuted.
+  // A wave's unit lies in one 32-row tile of weights, so gate or up is uniform.
+  // The offsets fit 32 bits: the host holds 256 rows of either to 4 GB.
+  const uint8_t* const a_tile = (const uint8_t*)p.a + (int64_t)m0 * a_row_bytes;
+  const uint8_t* const b_tile = p.b + (int64_t)n0 * (p.K / 2);
+  uint32_t a_at[C::AU], b_at[C::BU];
+  const uint8_t* b_from[C::BU];
 #pragma unroll
   for (int i = 0; i < C::AU; ++i) {
     const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
     const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
-    const int m = m0 + (int)(off / 128);
-    a_src[i] = (const uint8_t*)p.a + (int64_t)(m < p.M ? m : p.M - 1) * a_row_bytes + off % 128;
+    const int r = (int)(off / 128);
+    a_at[i] = (uint32_t)(m0 + r < p.M ? r : p.M - 1 - m0) * (uint32_t)a_row_bytes + off % 128;
   }
 #pragma unroll
   for (int i = 0; i < C::BU; ++i) {
     const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
     const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
-    b_src[i] = p.b + weight_row<GATED, WN>(n0, (int)(off / C::WB), p.N) * (p.K / 2) + off % C::WB;
+    const int r = weight_row<GATED, WN>(n0, (int)(off / C::WB), p.N);
+    b_at[i] = (uint32_t)r * (uint32_t)(p.K / 2) + off % C::WB;
+    const int first = (wave * 64 + i * C::kThreads) * 16 / C::WB;
+    b_from[i] = b_tile + (is_up<GATED, WN>(first) ? (int64_t)p.N * (p.K / 2) : 0);
   }
   const uint32_t a_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_a;
   const uint32_t b_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_b;
@@ -369,12 +382,12 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
     if ((t + 1) * C::KS <= p.K) {
 #pragma unroll
       for (int i = 0; i < C::AU; ++i)
-        load_lds16(a_src[i] + t * a_step,
-                   a_base + buf * C::kABytes + (uint32_t)(tid + i * C::kThreads) * 16);
+        load_lds16(a_tile + (int64_t)t * 128, a_at[i],
+                   a_base + buf * C::kABytes + (wave * 64 + i * C::kThreads) * 16);
 #pragma unroll
       for (int i = 0; i < C::BU; ++i)
-        load_lds16(b_src[i] + (int64_t)t * C::WB,
-                   b_base + buf * C::kBBytes + (uint32_t)(tid + i * C::kThreads) * 16);
+        load_lds16(b_from[i] + (int64_t)t * C::WB, b_at[i],
+                   b_base + buf * C::kBBytes + (wave * 64 + i * C::kThreads) * 16);
     } else {
       // the last step of a K that is no multiple of it: zeros behind the end
       const int left = p.K - t * C::KS;  // values
@@ -384,7 +397,7 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
         const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
         const bool in = (int)(off % 128) < left * (ACT == kFp8 ? 1 : 2);
         *(uint4*)(lds_a + buf * C::kABytes + dst) =
-            in ? *(const uint4*)(a_src[i] + t * a_step) : make_uint4(0, 0, 0, 0);
+            in ? *(const uint4*)(a_tile + a_at[i] + (int64_t)t * 128) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll
       for (int i = 0; i < C::BU; ++i) {
@@ -392,7 +405,7 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
         const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
         const bool in = (int)(off % C::WB) < left / 2;
         *(uint4*)(lds_b + buf * C::kBBytes + dst) =
-            in ? *(const uint4*)(b_src[i] + (int64_t)t * C::WB) : make_uint4(0, 0, 0, 0);
+            in ? *(const uint4*)(b_from[i] + b_at[i] + (int64_t)t * C::WB) : make_uint4(0, 0, 0, 0);
       }
     }
   };
@@ -405,7 +418,8 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
       if (r >= C::kSRows) break;
       const uint8_t* src;
       if (r < C::TN) {
-        src = p.b_scale + weight_row<GATED, WN>(n0, r, p.N) * blocks;
+        src = p.b_scale + (n0 + weight_row<GATED, WN>(n0, r, p.N) +
+                           (is_up<GATED, WN>(r) ? (int64_t)p.N : 0)) * blocks;
       } else {
         const int m = m0 + r - C::TN;
         src = p.a_scale + (int64_t)(m < p.M ? m : p.M - 1) * blocks;
@@ -419,7 +433,8 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
             const int at = u * 16 + j * 4 + k;
-            v[i][j] |= (at < blocks ? (uint32_t)src[at] : 127u) << (8 * k);
+            const uint32_t byte = src[at < blocks ? at : blocks - 1];
+            v[i][j] |= (at < blocks ? byte : 127u) << (8 * k);
           }
         }
       }
@@ -443,20 +458,31 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
 
   uint32_t sv[C::SU][4];
   scales(0, sv);
-  stage(0, 0);
   put_scales(0, sv);
+  stage(0, 0);
+  if (steps > 1) stage(1, 1);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
 
+  // Where a lane reads. Rows 32 apart have one permutation (tokens), so a byte
+  // of the row is flipped into the address and the tile of 32 is an offset.
   const int b_row = wn * WN * 32 + lr, a_row = wm * WM * 32 + lr;
+  const uint32_t read_a = lds_at<128>(a_row, 0);
+  uint32_t read_b[WN];
+#pragma unroll
+  for (int i = 0; i < WN; ++i) read_b[i] = lds_at<C::WB>(b_row + i * 32, 0) ^ (g * 16);
+  int buf = 0;
   for (int t = 0; t < steps; ++t) {
-    const int buf = t & 1, u = t / C::kSteps, s = t % C::kSteps;
+    const int u = t / C::kSteps, s = t % C::kSteps;
     const bool more = (u + 1) * 16 < blocks;
-    if (t + 1 < steps) stage(t + 1, buf ^ 1);
-    if (s == 0 && more) scales(u + 1, sv);
+    // Scales are written one step after they were asked for and before this
+    // step's loads: what the compiler waits for then is due anyway.
+    if (s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
+    if (s == C::kSteps - 2 && more) scales(u + 1, sv);
+    __builtin_amdgcn_sched_barrier(0);
+    if (t + 2 < steps) stage(t + 2, buf == 0 ? 2 : buf - 1);
 
-    const uint8_t* la = lds_a + buf * C::kABytes;
-    const uint8_t* lb = lds_b + buf * C::kBBytes;
+    const uint32_t at_a = read_a + buf * C::kABytes, at_b = buf * C::kBBytes;
     const uint32_t* ls = lds_s + ((u & 1) * 4 + s * 4 / C::kSteps) * C::kSRows;
     uint32_t ws[WN];
 #pragma unroll
@@ -471,11 +497,11 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
         uint4 w[WN];
 #pragma unroll
         for (int i = 0; i < WN; ++i)
-          w[i] = *(const uint4*)(lb + lds_at<C::WB>(b_row + i * 32, k * 32 + g * 16));
+          w[i] = *(const uint4*)(lds_b + at_b + (read_b[i] ^ (k * 32)));
 #pragma unroll
         for (int j = 0; j < WM; ++j) {
-          x[j].q[0] = *(const uint4*)(la + lds_at<128>(a_row + j * 32, k * 64 + g * 16));
-          x[j].q[1] = *(const uint4*)(la + lds_at<128>(a_row + j * 32, k * 64 + 32 + g * 16));
+          x[j].q[0] = *(const uint4*)(lds_a + (at_a ^ (k * 64 + g * 16)) + j * 4096);
+          x[j].q[1] = *(const uint4*)(lds_a + (at_a ^ (k * 64 + 32 + g * 16)) + j * 4096);
         }
 #pragma unroll
         for (int i = 0; i < WN; ++i) {
@@ -497,7 +523,7 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
       bool narrow = ACT == kFp16;
 #pragma unroll
       for (int i = 0; i < WN; ++i) {
-        w[i] = *(const uint4*)(lb + lds_at<C::WB>(b_row + i * 32, g * 16));
+        w[i] = *(const uint4*)(lds_b + at_b + read_b[i]);
         ws[i] = ws[i] >> (16 * (s & 1)) & 255u;  // two steps to a dword
       }
       if constexpr (ACT == kFp16) {
@@ -512,7 +538,7 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
           uint4 x[WM];
 #pragma unroll
           for (int j = 0; j < WM; ++j)
-            x[j] = *(const uint4*)(la + lds_at<128>(a_row + j * 32, g * 64 + k * 16));
+            x[j] = *(const uint4*)(lds_a + (at_a ^ (g * 64 + k * 16)) + j * 4096);
 #pragma unroll
           for (int i = 0; i < WN; ++i) {
             const uint32_t q = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
@@ -535,9 +561,10 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
         for (int k = 0; k < 4; ++k) {
 #pragma unroll
           for (int j = 0; j < WM; ++j) {
-            const uint4 x = *(const uint4*)(la + lds_at<128>(a_row + j * 32, g * 64 + k * 16));
+            const uint4 x = *(const uint4*)(lds_a + (at_a ^ (g * 64 + k * 16)) + j * 4096);
             bf16x8_t hi, lo;
             split_f16(x, hi, lo);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
             for (int i = 0; i < WN; ++i) {
               const uint32_t q = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
@@ -549,10 +576,12 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
         }
       }
     }
-    if (s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
-    // the buffers of the next step are full, and this step's are free
-    __builtin_amdgcn_s_waitcnt(0);
+    // Until the next step's buffer is full: the loads for the step after it
+    // stay in flight (the last step of a K that it does not divide has none).
+    if ((t + 3) * C::KS <= p.K) __builtin_amdgcn_s_waitcnt(C::kInFlight | 7 << 4);
+    else __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
+    buf = buf == 2 ? 0 : buf + 1;
   }
 
   // lane: token lr of a tile; register r: output (r & 3) + 8 (r >> 2) + 4 g
