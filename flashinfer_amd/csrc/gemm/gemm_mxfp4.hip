@@ -288,7 +288,6 @@ __device__ __forceinline__ uint32_t lds_at(int row, int byte) {
 template <int ACT, bool GATED, int WN, int WM, int GN, int GM>
 struct Tile {
   static constexpr int kThreads = GN * GM * 64;
-  static constexpr int kBufs = 3;
   static constexpr int TN = GN * WN * 32, TM = GM * WM * 32;
   static constexpr int kOut = GATED ? TN / 2 : TN;       // outputs of a tile along N
   static constexpr int KS = ACT == kFp8 ? 128 : 64;      // values of a step
@@ -296,7 +295,12 @@ struct Tile {
   static constexpr int kSteps = 512 / KS;                // steps of one load of scales
   static constexpr int kABytes = TM * 128, kBBytes = TN * WB;
   static constexpr int kSRows = TN + (ACT == kFp8 ? TM : 0);
-  static constexpr int kLds = kBufs * (kABytes + kBBytes) + 2 * 16 * kSRows;
+  static constexpr int kStage = kABytes + kBBytes, kScales = 2 * 16 * kSRows;
+  // a workgroup of four waves shares a CU with another
+  static constexpr int kMost = kThreads == 256 ? kLdsBytes / 2 : kLdsBytes;
+  static constexpr int kBufs = 3 * kStage + kScales <= kMost ? 3 : 2;
+  static constexpr int kLds = kBufs * kStage + kScales;
+  static_assert(kLds <= kMost, "");
   static constexpr int AU = kABytes / 16 / kThreads, BU = kBBytes / 16 / kThreads;
   static constexpr int kInFlight = AU + BU;              // loads a wave issues for a step
   static constexpr int SU = (kSRows + kThreads - 1) / kThreads;
@@ -329,7 +333,7 @@ __device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t at, uin
 }
 
 template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
-__global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_n, int tiles_m) {
+__global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int tiles_n, int tiles_m) {
   using C = Tile<ACT, GATED, WN, WM, GN, GM>;
   __shared__ __attribute__((aligned(256))) uint8_t lds[C::kLds];
   uint8_t* const lds_a = lds;
@@ -460,7 +464,7 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
   scales(0, sv);
   put_scales(0, sv);
   stage(0, 0);
-  if (steps > 1) stage(1, 1);
+  if (C::kBufs == 3 && steps > 1) stage(1, 1);
   __builtin_amdgcn_s_waitcnt(0);
   __syncthreads();
 
@@ -480,7 +484,7 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
     if (s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
     if (s == C::kSteps - 2 && more) scales(u + 1, sv);
     __builtin_amdgcn_sched_barrier(0);
-    if (t + 2 < steps) stage(t + 2, buf == 0 ? 2 : buf - 1);
+    if (t + C::kBufs - 1 < steps) stage(t + C::kBufs - 1, buf == 0 ? C::kBufs - 1 : buf - 1);
 
     const uint32_t at_a = read_a + buf * C::kABytes, at_b = buf * C::kBBytes;
     const uint32_t* ls = lds_s + ((u & 1) * 4 + s * 4 / C::kSteps) * C::kSRows;
@@ -533,12 +537,20 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
         narrow = __all(ok);
       }
       if (narrow || ACT == kBf16) {
+        // the next product's tokens are on their way while this one's multiply
+        uint4 x[2][WM];
+#pragma unroll
+        for (int j = 0; j < WM; ++j)
+          x[0][j] = *(const uint4*)(lds_a + (at_a ^ (g * 64)) + j * 4096);
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          uint4 x[WM];
+          if (k < 3) {
 #pragma unroll
-          for (int j = 0; j < WM; ++j)
-            x[j] = *(const uint4*)(lds_a + (at_a ^ (g * 64 + k * 16)) + j * 4096);
+            for (int j = 0; j < WM; ++j)
+              x[(k + 1) & 1][j] =
+                  *(const uint4*)(lds_a + (at_a ^ (g * 64 + (k + 1) * 16)) + j * 4096);
+          }
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int i = 0; i < WN; ++i) {
             const uint32_t q = k == 0 ? w[i].x : k == 1 ? w[i].y : k == 2 ? w[i].z : w[i].w;
@@ -546,12 +558,14 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
               const f16x8_t wv = widen_f16(q, scale_value(ws[i]));
 #pragma unroll
               for (int j = 0; j < WM; ++j)
-                acc[i][j] = mfma_32x32x16_f16(wv, __builtin_bit_cast(f16x8_t, x[j]), acc[i][j]);
+                acc[i][j] =
+                    mfma_32x32x16_f16(wv, __builtin_bit_cast(f16x8_t, x[k & 1][j]), acc[i][j]);
             } else {
               const bf16x8_t wv = widen_bf16(q, scale_value(ws[i]));
 #pragma unroll
               for (int j = 0; j < WM; ++j)
-                acc[i][j] = mfma_32x32x16_bf16(wv, __builtin_bit_cast(bf16x8_t, x[j]), acc[i][j]);
+                acc[i][j] =
+                    mfma_32x32x16_bf16(wv, __builtin_bit_cast(bf16x8_t, x[k & 1][j]), acc[i][j]);
             }
           }
         }
@@ -578,10 +592,10 @@ __global__ __launch_bounds__(GN * GM * 64) void tile_kernel(Params p, int tiles_
     }
     // Until the next step's buffer is full: the loads for the step after it
     // stay in flight (the last step of a K that it does not divide has none).
-    if ((t + 3) * C::KS <= p.K) __builtin_amdgcn_s_waitcnt(C::kInFlight | 7 << 4);
+    if (C::kBufs == 3 && (t + 3) * C::KS <= p.K) __builtin_amdgcn_s_waitcnt(C::kInFlight | 7 << 4);
     else __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
-    buf = buf == 2 ? 0 : buf + 1;
+    buf = buf == C::kBufs - 1 ? 0 : buf + 1;
   }
 
   // lane: token lr of a tile; register r: output (r & 3) + 8 (r >> 2) + 4 g
@@ -641,7 +655,7 @@ hipError_t launch_tile(const Params& p, hipStream_t stream) {
 
 template <int ACT, bool GATED, int OUT>
 hipError_t launch(const Params& p, hipStream_t stream) {
-  if (p.M > 64) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 2>(p, stream);
+  if (p.M > 64) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 1>(p, stream);
   constexpr int RT = OUT == kFp8 ? 2 : 1, MT = 1, WAVES = 4;
   dim3 grid(ceil_div(p.N, RT * 16), ceil_div(p.M, MT * 16));
   hipLaunchKernelGGL((rows_kernel<ACT, GATED, OUT, RT, MT, WAVES>), grid, dim3(WAVES * 64), 0,
