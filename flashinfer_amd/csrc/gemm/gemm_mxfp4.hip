@@ -46,17 +46,23 @@ enum { kBf16 = 0, kFp16 = 1, kFp8 = 2 };  // types of a
 typedef __attribute__((ext_vector_type(2))) __bf16 bf16x2_t;
 typedef __attribute__((ext_vector_type(2))) _Float16 f16x2_t;
 
+// g / (1 + 2^t): the exponential and the reciprocal of the hardware are off by
+// an ulp, and by |t| 2^-24 through t - far below a rounding to 16 bits. Where
+// 2^t overflows the reciprocal is 0.
+__device__ __forceinline__ float times_logistic(float g, float t) {
+  return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
+}
+
 template <int kAct>
 __device__ __forceinline__ float activate(float g) {
   if constexpr (kAct == 0) {
-    return g / (1.f + __builtin_expf(-g));
+    return times_logistic(g, g * -1.4426950408889634f);
   } else if constexpr (kAct == 1) {
     // erfc keeps the small negative tail that 1 + erf rounds away
     return 0.5f * g * erfcf(g * -0.70710678118654752f);
   } else {
-    // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u))
-    const float u = 0.79788456080286536f * (g + 0.044715f * g * g * g);
-    return g / (1.f + __builtin_expf(-2.f * u));
+    // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)), u = sqrt(2 / pi) (g + 0.044715 g^3)
+    return times_logistic(g, g * (-2.3022081985f - 0.1029432397f * g * g));
   }
 }
 
@@ -335,7 +341,10 @@ __device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t at, uin
 template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
 __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int tiles_n, int tiles_m) {
   using C = Tile<ACT, GATED, WN, WM, GN, GM>;
-  __shared__ __attribute__((aligned(256))) uint8_t lds[C::kLds];
+  constexpr int kSize = OUT == kFp8 ? 1 : 2;
+  constexpr int kRow = C::kOut * kSize + 16;  // of the outputs; the odd piece spreads the banks
+  constexpr int kShared = C::TM * kRow > C::kLds ? C::TM * kRow : C::kLds;
+  __shared__ __attribute__((aligned(256))) uint8_t lds[kShared];
   uint8_t* const lds_a = lds;
   uint8_t* const lds_b = lds + C::kBufs * C::kABytes;
   uint32_t* const lds_s = (uint32_t*)(lds + C::kBufs * (C::kABytes + C::kBBytes));  // [2][4][kSRows]
@@ -598,46 +607,82 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
     buf = buf == C::kBufs - 1 ? 0 : buf + 1;
   }
 
-  // lane: token lr of a tile; register r: output (r & 3) + 8 (r >> 2) + 4 g
+  // Through shared memory, so that a row of the tile leaves in 16-byte pieces.
+  // Lane: token lr of 32; register r: output (r & 3) + 8 (r >> 2) + 4 g.
+  constexpr int H = GATED ? WN / 2 : WN;
+  if constexpr (GATED) {
+    auto gate = [&](auto kind) {
+#pragma unroll
+      for (int i = 0; i < H; ++i)
+#pragma unroll
+        for (int j = 0; j < WM; ++j)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            acc[i][j][r] = activate<decltype(kind)::value>(acc[i][j][r]) * acc[i + H][j][r];
+    };
+    if (p.act == 0) gate(std::integral_constant<int, 0>());
+    else if (p.act == 1) gate(std::integral_constant<int, 1>());
+    else gate(std::integral_constant<int, 2>());
+  }
+  using T = typename std::conditional<OUT == kBf16, bf16, fp16>::type;
 #pragma unroll
   for (int j = 0; j < WM; ++j) {
-    const int m = m0 + a_row + j * 32;
-    constexpr int H = GATED ? WN / 2 : WN;
 #pragma unroll
     for (int i = 0; i < H; ++i) {
-      const int n = n0 + (wn * H + i) * 32 + 4 * g;
-      float y[16];
-#pragma unroll
-      for (int r = 0; r < 16; ++r)
-        y[r] = GATED ? activate(p.act, acc[i][j][r]) * acc[i + (GATED ? H : 0)][j][r]
-                     : acc[i][j][r];
+      const int nl = (wn * H + i) * 32 + 4 * g;
+      uint8_t* to = lds + (a_row + j * 32) * kRow + nl * kSize;
       if constexpr (OUT == kFp8) {
+        float y[16];
         uint32_t most = 0;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) most = abs_bits(y[r]) > most ? abs_bits(y[r]) : most;
+        for (int r = 0; r < 16; ++r) {
+          y[r] = acc[i][j][r];
+          most = abs_bits(y[r]) > most ? abs_bits(y[r]) : most;
+        }
         uint32_t a, b;
         permlane32_pair(most, most, a, b);  // the other half of the block
         most = a > b ? a : b;
         const uint32_t byte = mxfp8_scale_byte(most);
         const float inv = mx_inverse_scale(byte);
-        if (m < p.M && n - 4 * g < p.N) {
-          uint8_t* o = (uint8_t*)p.out + (int64_t)m * p.ldo + n;
 #pragma unroll
-          for (int r = 0; r < 16; r += 8) {
-            const uint2 q = mxfp8_pack8(y + r, inv, byte == 255u);
-            *(uint32_t*)(o + r * 2) = q.x;
-            *(uint32_t*)(o + r * 2 + 8) = q.y;
-          }
-          if (g == 0)
-            p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
+        for (int r = 0; r < 16; r += 8) {
+          const uint2 q = mxfp8_pack8(y + r, inv, byte == 255u);
+          *(uint32_t*)(to + r * 2) = q.x;
+          *(uint32_t*)(to + r * 2 + 8) = q.y;
         }
-      } else if (m < p.M) {
-        using T = typename std::conditional<OUT == kBf16, bf16, fp16>::type;
-        T* o = (T*)p.out + (int64_t)m * p.ldo + n;
+        const int m = m0 + a_row + j * 32, n = n0 + nl;
+        if (g == 0 && m < p.M && n < p.N)
+          p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
+      } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (n + (r & 3) + 8 * (r >> 2) < p.N) o[(r & 3) + 8 * (r >> 2)] = from_f32<T>(y[r]);
+        for (int r = 0; r < 16; r += 4) {
+          union { T v[4]; uint2 q; } y;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) y.v[k] = from_f32<T>(acc[i][j][r + k]);
+          *(uint2*)(to + r * 4) = y.q;
+        }
       }
+    }
+  }
+  __syncthreads();
+  constexpr int kPieces = C::kOut * kSize / 16, kEach = 16 / kSize;
+  const bool whole = ((uintptr_t)p.out % 16 | p.ldo * kSize % 16) == 0;
+  for (int i = tid; i < C::TM * kPieces; i += C::kThreads) {
+    const int ml = i / kPieces, nl = i % kPieces * kEach;
+    const int m = m0 + ml, n = n0 + nl;
+    if (m >= p.M || n >= p.N) continue;
+    const uint8_t* from = lds + ml * kRow + nl * kSize;
+    uint8_t* to = (uint8_t*)p.out + ((int64_t)m * p.ldo + n) * kSize;
+    if (whole && n + kEach <= p.N) {
+      *(uint4*)to = *(const uint4*)from;
+    } else if constexpr (OUT == kFp8) {
+      // rows at multiples of 8, N at one of 32
+      ((uint2*)to)[0] = ((const uint2*)from)[0];
+      ((uint2*)to)[1] = ((const uint2*)from)[1];
+    } else {
+#pragma unroll
+      for (int k = 0; k < kEach; ++k)
+        if (n + k < p.N) ((uint16_t*)to)[k] = ((const uint16_t*)from)[k];
     }
   }
 }
