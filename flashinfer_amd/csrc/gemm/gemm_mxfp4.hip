@@ -112,109 +112,235 @@ __device__ __forceinline__ bool f16_exact(uint32_t byte) {
   return byte >= 104u && byte <= 140u;
 }
 
-// WAVES waves share a tile of RT * 16 outputs by MT * 16 tokens and take the
-// chunks of K in turn; their sums are joined in a fixed order.
-template <int ACT, bool GATED, int OUT, int RT, int MT, int WAVES>
-__global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
-  constexpr int AT = GATED ? 2 * RT : RT;  // weight tiles
-  constexpr int LD = AT * 16 + 4;
-  __shared__ __attribute__((aligned(16))) float red[WAVES][MT * 16][LD];
+// ---------------------------------------------------------------------------
+// Loads to shared memory, and the waits for them.
 
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// 16 bytes a lane to the wave's 1024 at `dst` (a wave's own, uniform address).
+// In assembly, for the compiler holds every read of shared memory behind such
+// a load, also where the two go to different buffers: with the builtin the
+// next step's loads were waited for before this step's products. Nothing waits
+// for it here: the callers count these loads.
+__device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
+               :
+               : "s"(dst), "v"(src)
+               : "memory");
+}
+__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t at, uint32_t dst) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               :
+               : "s"(dst), "v"(at), "s"(base)
+               : "memory");
+}
+
+__device__ __forceinline__ uint32_t lds_address(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;
+}
+
+// s_waitcnt for at most `vm` loads, and for shared memory too where `lds`
+constexpr int wait_code(int vm, bool lds) {
+  return (vm & 15) | (vm >> 4) << 14 | 7 << 4 | (lds ? 0 : 15) << 8;
+}
+
+// until all but the newest `stages` of a wave's stages, kOps loads each, are in
+template <int kOps, int kMost>
+__device__ __forceinline__ void wait_stages(int stages) {
+  static_assert(kOps * kMost < 64, "");
+  if constexpr (kMost > 0) {
+    if (stages >= kMost) __builtin_amdgcn_s_waitcnt(wait_code(kOps * kMost, false));
+    else wait_stages<kOps, kMost - 1>(stages);
+  } else {
+    __builtin_amdgcn_s_waitcnt(wait_code(0, false));
+  }
+}
+
+// 16-byte units spread over the banks: of rows of 32 to 256 bytes, a column of
+// 16 or 32 rows is then read without conflicts
+__device__ __forceinline__ uint32_t spread(uint32_t off) {
+  return off ^ (((off >> 8) & 15) << 4);
+}
+
+// ---------------------------------------------------------------------------
+// Few tokens (16 at most): the weights' bytes are what the time goes to, and
+// how many of them are on their way at once decides how fast they come. A
+// workgroup of WAVES waves takes RT * 16 outputs and shares K among its waves
+// in chunks of 128. Each wave has D chunks of weights (AT KB) and tokens (XI
+// KB) on their way to its own part of shared memory, by loads that bypass the
+// registers, and waits for the oldest alone: there is no barrier in the loop.
+// The scales of a slab of K are read ahead of it. The waves' sums are joined
+// in a fixed order.
+template <int ACT, bool GATED, int RT, int XI, int WAVES, int D>
+struct Rows {
+  static constexpr int AT = GATED ? 2 * RT : RT;             // tiles of 16 weight rows
+  static constexpr int kXRow = ACT == kFp8 ? 128 : 256;      // bytes of a token in a chunk
+  static constexpr int MR = XI * 1024 / kXRow;               // tokens held, 16 at most
+  static constexpr int kStage = (AT + XI) * 1024;
+  static constexpr int kSlab = 192;                          // blocks of K with resident scales
+  static constexpr int kSRow = kSlab + 4;                    // one word more: rows in unlike banks
+  static constexpr int kSRows = AT * 16 + (ACT == kFp8 ? MR : 0);
+  static constexpr int LD = AT * 16 + 4;                     // of the sums to be joined
+  static constexpr int kRing = WAVES * D * kStage;
+  static constexpr int kJoin = WAVES * 16 * LD * 4;
+  static constexpr int kLds = kRing + kSRows * kSRow > kJoin ? kRing + kSRows * kSRow : kJoin;
+  static constexpr int kWavesPerSimd = WAVES / 4 * (kLdsBytes / kLds < 2 ? 1 : 2);
+  static_assert(MR <= 16 && kLds <= kLdsBytes, "");
+};
+
+template <int ACT, bool GATED, int OUT, int RT, int XI, int WAVES, int D>
+__global__ __launch_bounds__(WAVES * 64, (Rows<ACT, GATED, RT, XI, WAVES, D>::kWavesPerSimd))
+void rows_kernel(Params p) {
+  using C = Rows<ACT, GATED, RT, XI, WAVES, D>;
+  constexpr int AT = C::AT;
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
+  uint8_t* const lds_s = lds + C::kRing;
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * RT * 16, m0 = blockIdx.y * MT * 16;
+  const int n0 = blockIdx.x * RT * 16;
   const int blocks = p.K / kMxBlock;
 
-  const uint8_t* brow[AT];
-  const uint8_t* srow[AT];
+  auto weight_at = [&](int r) {  // the weight row of row r of the AT tiles
+    const int n = n0 + r % (RT * 16);
+    return (n < p.N ? n : p.N - 1) + (r >= RT * 16 ? (int64_t)p.N : 0);
+  };
+  // lane l brings unit l of a kilobyte: the place is linear, the source permuted
+  const uint32_t b_unit = spread(lane * 16);
+  const uint8_t* b_src[AT];
 #pragma unroll
-  for (int t = 0; t < AT; ++t) {
-    const int n = n0 + (t % RT) * 16 + lr;
-    const int64_t row = (n < p.N ? n : p.N - 1) + (t >= RT ? (int64_t)p.N : 0);
-    brow[t] = p.b + row * (p.K / 2);
-    srow[t] = p.b_scale + row * blocks;
+  for (int t = 0; t < AT; ++t)
+    b_src[t] = p.b + weight_at(t * 16 + (int)(b_unit / 64)) * (p.K / 2);
+  const uint8_t* x_src[XI];
+#pragma unroll
+  for (int i = 0; i < XI; ++i) {
+    const int r = (int)(spread(i * 1024 + lane * 16) / C::kXRow);
+    x_src[i] = (const uint8_t*)p.a +
+               (int64_t)(r < p.M ? r : p.M - 1) * p.lda * (ACT == kFp8 ? 1 : 2);
   }
-  int64_t arow[MT];
-#pragma unroll
-  for (int t = 0; t < MT; ++t) {
-    const int m = m0 + t * 16 + lr;
-    arow[t] = m < p.M ? m : p.M - 1;
-  }
+  const uint32_t ring = lds_address(lds) + wave * D * C::kStage;
+  const uint8_t* const ring_p = lds + wave * D * C::kStage;
 
-  floatx4 acc[AT][MT];
+  // chunk c of K to place `slot` of the wave's ring. Behind the end of a row
+  // its last unit comes again: those values are cleared where they are used.
+  auto stage = [&](int c, int slot) {
+    const uint32_t to = ring + slot * C::kStage;
+    const int b_last = p.K / 2 - 16, x_last = p.K * (ACT == kFp8 ? 1 : 2) - 16;
+    const int b_off = c * 64 + (int)(b_unit % 64);
 #pragma unroll
-  for (int i = 0; i < AT; ++i)
+    for (int t = 0; t < AT; ++t)
+      load_lds16(b_src[t] + (b_off < b_last ? b_off : b_last), to + t * 1024);
 #pragma unroll
-    for (int j = 0; j < MT; ++j) acc[i][j] = floatx4{0.f, 0.f, 0.f, 0.f};
-
-  for (int c = wave * 4; c < blocks; c += WAVES * 4) {
-    const int kb = c + g;
-    const bool in = kb < blocks;
-    uint4 w[AT];
-    uint32_t ws[AT];
-#pragma unroll
-    for (int t = 0; t < AT; ++t) {
-      w[t] = in ? *reinterpret_cast<const uint4*>(brow[t] + (int64_t)kb * 16)
-                : make_uint4(0, 0, 0, 0);
-      ws[t] = in ? srow[t][kb] : 127u;
+    for (int i = 0; i < XI; ++i) {
+      const int x_off = c * C::kXRow + (int)(spread(i * 1024 + lane * 16) % C::kXRow);
+      load_lds16(x_src[i] + (x_off < x_last ? x_off : x_last), to + (AT + i) * 1024);
     }
-    if constexpr (ACT == kFp8) {
+  };
+
+  // where a lane reads: its weights' block, and its token's values. A column
+  // of no token reads some other token; its sums are not used.
+  const uint32_t read_b = spread(lr * 64 + g * 16);
+  const int xr = lr & (C::MR - 1);
+
+  floatx4 acc[AT];
 #pragma unroll
-      for (int j = 0; j < MT; ++j) {
-        const uint8_t* ap = (const uint8_t*)p.a + arow[j] * p.lda + c * 32 + g * 16;
-        union { intx8 v; uint4 q[2]; } u;
-        u.q[0] = c + (g >> 1) < blocks ? *reinterpret_cast<const uint4*>(ap)
-                                       : make_uint4(0, 0, 0, 0);
-        u.q[1] = c + 2 + (g >> 1) < blocks ? *reinterpret_cast<const uint4*>(ap + 64)
-                                           : make_uint4(0, 0, 0, 0);
-        const uint32_t as = in ? p.a_scale[arow[j] * blocks + kb] : 127u;
+  for (int t = 0; t < AT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+
+  for (int s0 = 0; s0 < blocks; s0 += C::kSlab) {
+    const int width = blocks - s0 < C::kSlab ? blocks - s0 : C::kSlab;
+    const int c0 = s0 / 4, chunks = (width + 3) / 4;
+    // this wave's chunks of the slab: c0 + wave, and every WAVES further
+    const int mine = chunks > wave ? (chunks - wave - 1) / WAVES + 1 : 0;
+#pragma unroll
+    for (int i = 0; i < D; ++i)
+      if (i < mine) stage(c0 + wave + i * WAVES, i);
+
+    // the slab's scales, four to a word; NaN-free ones behind its end
+    if (s0) __syncthreads();  // the slab before this one is done with its scales
+    for (int i = tid; i < C::kSRows * (C::kSlab / 4); i += WAVES * 64) {
+      const int r = i / (C::kSlab / 4), at = i % (C::kSlab / 4) * 4;
+      if (at >= width) continue;
+      const uint8_t* src = r < AT * 16 ? p.b_scale + weight_at(r) * blocks + s0
+                                       : p.a_scale + (int64_t)(r - AT * 16 < p.M ? r - AT * 16 : p.M - 1) * blocks + s0;
+      uint32_t v = 0x7f7f7f7fu;
+      if (at + 4 <= width) __builtin_memcpy(&v, src + at, 4);
+      else for (int k = 0; k < width - at; ++k)
+        v = (v & ~(255u << 8 * k)) | (uint32_t)src[at + k] << 8 * k;
+      *(uint32_t*)(lds_s + r * C::kSRow + at) = v;
+    }
+    __syncthreads();
+
+    int slot = 0;
+    for (int i = 0; i < mine; ++i) {
+      const int c = wave + i * WAVES;  // in the slab
+      wait_stages<AT + XI, D - 1>(mine - 1 - i);
+      asm volatile("" ::: "memory");  // no read moves before the wait
+      const uint8_t* from = ring_p + slot * C::kStage;
+      uint4 w[AT];
+      uint32_t ws[AT];
+#pragma unroll
+      for (int t = 0; t < AT; ++t) {
+        w[t] = *(const uint4*)(from + t * 1024 + read_b);
+        ws[t] = lds_s[(t * 16 + lr) * C::kSRow + c * 4 + g];
+      }
+      constexpr int XU = ACT == kFp8 ? 2 : 4;  // 16-byte units of a token a lane takes
+      uint4 x[XU];
+      uint32_t xs = 127;
+#pragma unroll
+      for (int k = 0; k < XU; ++k) {
+        const int byte = ACT == kFp8 ? g * 16 + k * 64 : g * 64 + k * 16;
+        x[k] = *(const uint4*)(from + AT * 1024 + spread(xr * C::kXRow + byte));
+      }
+      if constexpr (ACT == kFp8) xs = lds_s[(AT * 16 + xr) * C::kSRow + c * 4 + g];
+      // all read: the place may be filled again
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      if (i + D < mine) stage(c0 + c + D * WAVES, slot);
+      slot = slot == D - 1 ? 0 : slot + 1;
+
+      if (c * 4 + 4 > width) {  // the last chunk of a K that 128 does not divide
+        const int left = width - c * 4;
+#pragma unroll
+        for (int t = 0; t < AT; ++t)
+          if (g >= left) w[t] = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < XU; ++k)
+          if ((ACT == kFp8 ? k * 2 + g / 2 : g) >= left) x[k] = make_uint4(0, 0, 0, 0);
+      }
+      if constexpr (ACT == kFp8) {
+        const intx8 xv = {(int)x[0].x, (int)x[0].y, (int)x[0].z, (int)x[0].w,
+                          (int)x[1].x, (int)x[1].y, (int)x[1].z, (int)x[1].w};
 #pragma unroll
         for (int t = 0; t < AT; ++t) {
-          intx8 wv = {(int)w[t].x, (int)w[t].y, (int)w[t].z, (int)w[t].w, 0, 0, 0, 0};
-          acc[t][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
-              wv, u.v, acc[t][j], 4, 0, 0, (int)ws[t], 0, (int)as);
+          const intx8 wv = {(int)w[t].x, (int)w[t].y, (int)w[t].z, (int)w[t].w, 0, 0, 0, 0};
+          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[t], 4, 0, 0,
+                                                                    (int)ws[t], 0, (int)xs);
         }
-      }
-    } else {
-      bool narrow = ACT == kFp16;
-      if constexpr (ACT == kFp16) {
-        bool ok = true;
+      } else {
+        bool narrow = ACT == kFp16;
+        if constexpr (ACT == kFp16) {
+          bool ok = true;
 #pragma unroll
-        for (int t = 0; t < AT; ++t) ok = ok && f16_exact(ws[t]);
-        narrow = __all(ok);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint4 x[MT];
-#pragma unroll
-        for (int j = 0; j < MT; ++j) {
-          const uint16_t* ap = (const uint16_t*)p.a + arow[j] * p.lda + (int64_t)kb * 32 + i * 8;
-          x[j] = in ? *reinterpret_cast<const uint4*>(ap) : make_uint4(0, 0, 0, 0);
+          for (int t = 0; t < AT; ++t) ok = ok && f16_exact(ws[t]);
+          narrow = __all(ok);
         }
-        if (narrow) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          bf16x8_t hi, lo;
+          if (ACT == kFp16 && !narrow) split_f16(x[k], hi, lo);
 #pragma unroll
           for (int t = 0; t < AT; ++t) {
-            const uint32_t q = i == 0 ? w[t].x : i == 1 ? w[t].y : i == 2 ? w[t].z : w[t].w;
-            const f16x8_t wv = widen_f16(q, scale_value(ws[t]));
-#pragma unroll
-            for (int j = 0; j < MT; ++j)
-              acc[t][j] = mfma_16x16x32_f16(wv, __builtin_bit_cast(f16x8_t, x[j]), acc[t][j]);
-          }
-        } else {
-          bf16x8_t hi[MT], lo[MT];
-#pragma unroll
-          for (int j = 0; j < MT; ++j) {
-            if constexpr (ACT == kFp16) split_f16(x[j], hi[j], lo[j]);
-            else hi[j] = __builtin_bit_cast(bf16x8_t, x[j]);
-          }
-#pragma unroll
-          for (int t = 0; t < AT; ++t) {
-            const uint32_t q = i == 0 ? w[t].x : i == 1 ? w[t].y : i == 2 ? w[t].z : w[t].w;
-            const bf16x8_t wv = widen_bf16(q, scale_value(ws[t]));
-#pragma unroll
-            for (int j = 0; j < MT; ++j) {
-              acc[t][j] = mfma_16x16x32_bf16(wv, hi[j], acc[t][j]);
-              if constexpr (ACT == kFp16) acc[t][j] = mfma_16x16x32_bf16(wv, lo[j], acc[t][j]);
+            const uint32_t q = k == 0 ? w[t].x : k == 1 ? w[t].y : k == 2 ? w[t].z : w[t].w;
+            if constexpr (ACT == kFp16) {
+              if (narrow) {
+                acc[t] = mfma_16x16x32_f16(widen_f16(q, scale_value(ws[t])),
+                                           __builtin_bit_cast(f16x8_t, x[k]), acc[t]);
+              } else {
+                const bf16x8_t wv = widen_bf16(q, scale_value(ws[t]));
+                acc[t] = mfma_16x16x32_bf16(wv, hi, acc[t]);
+                acc[t] = mfma_16x16x32_bf16(wv, lo, acc[t]);
+              }
+            } else {
+              acc[t] = mfma_16x16x32_bf16(widen_bf16(q, scale_value(ws[t])),
+                                          __builtin_bit_cast(bf16x8_t, x[k]), acc[t]);
             }
           }
         }
@@ -222,32 +348,29 @@ __global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
     }
   }
 
-  // every lane's sums are needed below, also where its column is no token
+  // Join the waves' sums. Every lane writes its own, also where its column is
+  // no token: an operand of a product may not sink into a branch.
+  __syncthreads();
+  float* const join = (float*)lds;
 #pragma unroll
   for (int t = 0; t < AT; ++t)
-#pragma unroll
-    for (int j = 0; j < MT; ++j)
-      *reinterpret_cast<floatx4*>(&red[wave][j * 16 + lr][t * 16 + g * 4]) = acc[t][j];
+    *(floatx4*)(join + (wave * 16 + lr) * C::LD + t * 16 + g * 4) = acc[t];
   __syncthreads();
 
   // eight neighbouring outputs of one token to a thread
   constexpr int G8 = RT * 2;
-  for (int i = threadIdx.x; i < MT * 16 * G8; i += WAVES * 64) {
-    const int ml = i / G8, nl = (i % G8) * 8;
-    const int m = m0 + ml, n = n0 + nl;
+  for (int i = tid; i < 16 * G8; i += WAVES * 64) {
+    const int m = i / G8, nl = (i % G8) * 8, n = n0 + nl;
     float y[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      float s = 0.f;
+      float s = 0.f, u = 0.f;
 #pragma unroll
-      for (int wv = 0; wv < WAVES; ++wv) s += red[wv][ml][nl + j];
-      if constexpr (GATED) {
-        float u = 0.f;
-#pragma unroll
-        for (int wv = 0; wv < WAVES; ++wv) u += red[wv][ml][RT * 16 + nl + j];
-        s = activate(p.act, s) * u;
+      for (int w = 0; w < WAVES; ++w) {
+        s += join[(w * 16 + m) * C::LD + nl + j];
+        if constexpr (GATED) u += join[(w * 16 + m) * C::LD + RT * 16 + nl + j];
       }
-      y[j] = s;
+      y[j] = GATED ? activate(p.act, s) * u : s;
     }
     if constexpr (OUT == kFp8) {
       // N is a multiple of 32 here and a quad holds one block
@@ -272,6 +395,13 @@ __global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
   }
 }
 
+template <int ACT, bool GATED, int OUT, int RT, int XI, int WAVES, int D>
+hipError_t launch_rows(const Params& p, hipStream_t stream) {
+  hipLaunchKernelGGL((rows_kernel<ACT, GATED, OUT, RT, XI, WAVES, D>),
+                     dim3(ceil_div(p.N, RT * 16)), dim3(WAVES * 64), 0, stream, p);
+  return hipGetLastError();
+}
+
 // ---------------------------------------------------------------------------
 // Many tokens: a workgroup of GN x GM waves computes a tile of GN * WN * 32
 // weight rows by GM * WM * 32 tokens in 32x32 products. Steps of 128 bytes of
@@ -284,12 +414,6 @@ __global__ __launch_bounds__(WAVES * 64) void rows_kernel(Params p) {
 //     lane group g supplies the scale of block g.
 //   16-bit a, 32x32x16, product i of 4 in a step: k = 32g + 8i .. 32g + 8i + 7,
 //     so that a lane's weights are one block of one scale here as well.
-
-template <int WB>  // bytes of a row in the buffer: 16-byte units spread over the banks
-__device__ __forceinline__ uint32_t lds_at(int row, int byte) {
-  const uint32_t off = (uint32_t)(row * WB + byte);
-  return off ^ (((off >> 8) & 15) << 4);
-}
 
 template <int ACT, bool GATED, int WN, int WM, int GN, int GM>
 struct Tile {
@@ -324,18 +448,6 @@ template <bool GATED, int WN>
 __device__ __forceinline__ int weight_row(int n0, int r, int N) {
   if constexpr (GATED) r = (r / (WN * 32) * (WN / 2) + r / 32 % (WN / 2)) * 32 + r % 32;
   return n0 + r < N ? r : N - 1 - n0;
-}
-
-// 16 bytes a lane from base + at to the wave's 1024 at `dst` (a wave's own, uniform
-// address). In assembly, for the compiler holds every read of shared memory
-// behind such a load, also where the two go to different buffers: with the
-// builtin the next step's loads were waited for before this step's products.
-// Nothing waits for it here: s_waitcnt vmcnt before the barrier does.
-__device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t at, uint32_t dst) {
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-               :
-               : "s"(dst), "v"(at), "s"(base)
-               : "memory");
 }
 
 template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
@@ -375,21 +487,21 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
 #pragma unroll
   for (int i = 0; i < C::AU; ++i) {
     const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
-    const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+    const uint32_t off = spread(dst);
     const int r = (int)(off / 128);
     a_at[i] = (uint32_t)(m0 + r < p.M ? r : p.M - 1 - m0) * (uint32_t)a_row_bytes + off % 128;
   }
 #pragma unroll
   for (int i = 0; i < C::BU; ++i) {
     const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
-    const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+    const uint32_t off = spread(dst);
     const int r = weight_row<GATED, WN>(n0, (int)(off / C::WB), p.N);
     b_at[i] = (uint32_t)r * (uint32_t)(p.K / 2) + off % C::WB;
     const int first = (wave * 64 + i * C::kThreads) * 16 / C::WB;
     b_from[i] = b_tile + (is_up<GATED, WN>(first) ? (int64_t)p.N * (p.K / 2) : 0);
   }
-  const uint32_t a_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_a;
-  const uint32_t b_base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds_b;
+  const uint32_t a_base = lds_address(lds_a);
+  const uint32_t b_base = lds_address(lds_b);
 
   auto stage = [&](int t, int buf) {
     if ((t + 1) * C::KS <= p.K) {
@@ -407,7 +519,7 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
 #pragma unroll
       for (int i = 0; i < C::AU; ++i) {
         const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
-        const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+        const uint32_t off = spread(dst);
         const bool in = (int)(off % 128) < left * (ACT == kFp8 ? 1 : 2);
         *(uint4*)(lds_a + buf * C::kABytes + dst) =
             in ? *(const uint4*)(a_tile + a_at[i] + (int64_t)t * 128) : make_uint4(0, 0, 0, 0);
@@ -415,7 +527,7 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
 #pragma unroll
       for (int i = 0; i < C::BU; ++i) {
         const uint32_t dst = (uint32_t)(tid + i * C::kThreads) * 16;
-        const uint32_t off = dst ^ (((dst >> 8) & 15) << 4);
+        const uint32_t off = spread(dst);
         const bool in = (int)(off % C::WB) < left / 2;
         *(uint4*)(lds_b + buf * C::kBBytes + dst) =
             in ? *(const uint4*)(b_from[i] + b_at[i] + (int64_t)t * C::WB) : make_uint4(0, 0, 0, 0);
@@ -480,10 +592,10 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
   // Where a lane reads. Rows 32 apart have one permutation (tokens), so a byte
   // of the row is flipped into the address and the tile of 32 is an offset.
   const int b_row = wn * WN * 32 + lr, a_row = wm * WM * 32 + lr;
-  const uint32_t read_a = lds_at<128>(a_row, 0);
+  const uint32_t read_a = spread(a_row * 128);
   uint32_t read_b[WN];
 #pragma unroll
-  for (int i = 0; i < WN; ++i) read_b[i] = lds_at<C::WB>(b_row + i * 32, 0) ^ (g * 16);
+  for (int i = 0; i < WN; ++i) read_b[i] = spread((b_row + i * 32) * C::WB) ^ (g * 16);
   int buf = 0;
   for (int t = 0; t < steps; ++t) {
     const int u = t / C::kSteps, s = t % C::kSteps;
@@ -601,7 +713,7 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
     }
     // Until the next step's buffer is full: the loads for the step after it
     // stay in flight (the last step of a K that it does not divide has none).
-    if (C::kBufs == 3 && (t + 3) * C::KS <= p.K) __builtin_amdgcn_s_waitcnt(C::kInFlight | 7 << 4);
+    if (C::kBufs == 3 && (t + 3) * C::KS <= p.K) __builtin_amdgcn_s_waitcnt(wait_code(C::kInFlight, true));
     else __builtin_amdgcn_s_waitcnt(0);
     __syncthreads();
     buf = buf == C::kBufs - 1 ? 0 : buf + 1;
@@ -700,12 +812,11 @@ hipError_t launch_tile(const Params& p, hipStream_t stream) {
 
 template <int ACT, bool GATED, int OUT>
 hipError_t launch(const Params& p, hipStream_t stream) {
-  if (p.M > 64) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 1>(p, stream);
-  constexpr int RT = OUT == kFp8 ? 2 : 1, MT = 1, WAVES = 4;
-  dim3 grid(ceil_div(p.N, RT * 16), ceil_div(p.M, MT * 16));
-  hipLaunchKernelGGL((rows_kernel<ACT, GATED, OUT, RT, MT, WAVES>), grid, dim3(WAVES * 64), 0,
-                     stream, p);
-  return hipGetLastError();
+  if (p.M > 16) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 1>(p, stream);
+  constexpr int RT = OUT == kFp8 ? 2 : 1;
+  constexpr int kFew = ACT == kFp8 ? 8 : 4;  // tokens in a kilobyte of a chunk
+  if (p.M <= kFew) return launch_rows<ACT, GATED, OUT, RT, 1, 8, GATED ? 3 : 4>(p, stream);
+  return launch_rows<ACT, GATED, OUT, RT, ACT == kFp8 ? 2 : 4, 8, OUT == kFp8 ? 2 : 3>(p, stream);
 }
 
 template <int ACT>
