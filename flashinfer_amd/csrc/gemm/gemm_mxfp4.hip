@@ -38,6 +38,7 @@ struct Params {
   int M, N, K;
   int64_t lda, ldo;
   int act;
+  float* sums;  // of the parts of K, where a product is split over it
 };
 
 enum { kBf16 = 0, kFp16 = 1, kFp8 = 2 };  // types of a
@@ -160,6 +161,26 @@ __device__ __forceinline__ uint32_t spread(uint32_t off) {
   return off ^ (((off >> 8) & 15) << 4);
 }
 
+// Scales at .. at + 15 of a row's `count`: 16 unaligned bytes, or what is left
+// of them and 127 (the scale 1) behind the end.
+__device__ __forceinline__ void load_scales(uint32_t (&v)[4], const uint8_t* row, int at,
+                                            int count) {
+  if (at + 16 <= count) {
+    __builtin_memcpy(v, row + at, 16);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      v[j] = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = at + j * 4 + k;
+        const uint32_t byte = row[i < count ? i : count - 1];
+        v[j] |= (i < count ? byte : 127u) << (8 * k);
+      }
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------
 // Few tokens (16 at most): the weights' bytes are what the time goes to, and
 // how many of them are on their way at once decides how fast they come. A
@@ -176,7 +197,7 @@ struct Rows {
   static constexpr int MR = XI * 1024 / kXRow;               // tokens held, 16 at most
   static constexpr int kStage = (AT + XI) * 1024;
   static constexpr int kSlab = 192;                          // blocks of K with resident scales
-  static constexpr int kSRow = kSlab + 4;                    // one word more: rows in unlike banks
+  static constexpr int kSRow = kSlab + 16;                   // one unit more: rows in unlike banks
   static constexpr int kSRows = AT * 16 + (ACT == kFp8 ? MR : 0);
   static constexpr int LD = AT * 16 + 4;                     // of the sums to be joined
   static constexpr int kRing = WAVES * D * kStage;
@@ -250,22 +271,31 @@ void rows_kernel(Params p) {
     const int c0 = s0 / 4, chunks = (width + 3) / 4;
     // this wave's chunks of the slab: c0 + wave, and every WAVES further
     const int mine = chunks > wave ? (chunks - wave - 1) / WAVES + 1 : 0;
+    // The slab's scales, 16 to a load: they are asked for before they are
+    // written, all at once. Behind the slab's end lies 127, which is 1.
+    constexpr int kUnits = C::kSRows * (C::kSlab / 16);
+    constexpr int kEach = (kUnits + WAVES * 64 - 1) / (WAVES * 64);
+    uint32_t sv[kEach][4];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = tid + j * WAVES * 64;
+      const int r = i / (C::kSlab / 16), at = i % (C::kSlab / 16) * 16;
+      if (i >= kUnits || at >= width) continue;
+      const uint8_t* src =
+          r < AT * 16 ? p.b_scale + weight_at(r) * blocks + s0
+                      : p.a_scale + (int64_t)(r - AT * 16 < p.M ? r - AT * 16 : p.M - 1) * blocks + s0;
+      load_scales(sv[j], src, at, width);
+    }
 #pragma unroll
     for (int i = 0; i < D; ++i)
       if (i < mine) stage(c0 + wave + i * WAVES, i);
-
-    // the slab's scales, four to a word; NaN-free ones behind its end
     if (s0) __syncthreads();  // the slab before this one is done with its scales
-    for (int i = tid; i < C::kSRows * (C::kSlab / 4); i += WAVES * 64) {
-      const int r = i / (C::kSlab / 4), at = i % (C::kSlab / 4) * 4;
-      if (at >= width) continue;
-      const uint8_t* src = r < AT * 16 ? p.b_scale + weight_at(r) * blocks + s0
-                                       : p.a_scale + (int64_t)(r - AT * 16 < p.M ? r - AT * 16 : p.M - 1) * blocks + s0;
-      uint32_t v = 0x7f7f7f7fu;
-      if (at + 4 <= width) __builtin_memcpy(&v, src + at, 4);
-      else for (int k = 0; k < width - at; ++k)
-        v = (v & ~(255u << 8 * k)) | (uint32_t)src[at + k] << 8 * k;
-      *(uint32_t*)(lds_s + r * C::kSRow + at) = v;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const int i = tid + j * WAVES * 64;
+      const int r = i / (C::kSlab / 16), at = i % (C::kSlab / 16) * 16;
+      if (i >= kUnits || at >= width) continue;
+      *(uint4*)(lds_s + r * C::kSRow + at) = make_uint4(sv[j][0], sv[j][1], sv[j][2], sv[j][3]);
     }
     __syncthreads();
 
@@ -406,7 +436,7 @@ hipError_t launch_rows(const Params& p, hipStream_t stream) {
 // Many tokens: a workgroup of GN x GM waves computes a tile of GN * WN * 32
 // weight rows by GM * WM * 32 tokens in 32x32 products. Steps of 128 bytes of
 // a token row (128 values in 8 bits, 64 in 16) go to shared memory with their
-// weights, three buffers in turn, by loads that bypass the registers; the scales
+// weights, several buffers in turn, by loads that bypass the registers; the scales
 // of 512 values of a row come as 16 bytes once per 512.
 //
 // Operand map of 32x32: lane l holds row (token) l & 31 and, with g = l >> 5,
@@ -417,7 +447,13 @@ hipError_t launch_rows(const Params& p, hipStream_t stream) {
 
 template <int ACT, bool GATED, int WN, int WM, int GN, int GM>
 struct Tile {
-  static constexpr int kThreads = GN * GM * 64;
+  static constexpr int kThreads = GN * GM * 64;          // that multiply
+  // Small tiles wait for memory rather than for the matrix unit: a wave more
+  // brings the scales, so that no other wave's wait for its scales is a wait
+  // for all the steps that it has asked for since.
+  static constexpr bool kHelper = WN * WM <= 4;
+  static constexpr int kLaunch = kThreads + (kHelper ? 64 : 0);
+  static constexpr int kScaleThreads = kHelper ? 64 : kThreads;
   static constexpr int TN = GN * WN * 32, TM = GM * WM * 32;
   static constexpr int kOut = GATED ? TN / 2 : TN;       // outputs of a tile along N
   static constexpr int KS = ACT == kFp8 ? 128 : 64;      // values of a step
@@ -428,12 +464,14 @@ struct Tile {
   static constexpr int kStage = kABytes + kBBytes, kScales = 2 * 16 * kSRows;
   // a workgroup of four waves shares a CU with another
   static constexpr int kMost = kThreads == 256 ? kLdsBytes / 2 : kLdsBytes;
-  static constexpr int kBufs = 3 * kStage + kScales <= kMost ? 3 : 2;
+  static constexpr int kFit = (kMost - kScales) / kStage;
+  static constexpr int kBufs = kFit < 8 ? kFit : 8;
+  static constexpr int kAhead = kBufs - 1;               // steps on their way
   static constexpr int kLds = kBufs * kStage + kScales;
-  static_assert(kLds <= kMost, "");
+  static_assert(kBufs >= 2, "");
   static constexpr int AU = kABytes / 16 / kThreads, BU = kBBytes / 16 / kThreads;
   static constexpr int kInFlight = AU + BU;              // loads a wave issues for a step
-  static constexpr int SU = (kSRows + kThreads - 1) / kThreads;
+  static constexpr int SU = (kSRows + kScaleThreads - 1) / kScaleThreads;
   static_assert(AU * 16 * kThreads == kABytes && BU * 16 * kThreads == kBBytes, "");
 };
 
@@ -451,7 +489,9 @@ __device__ __forceinline__ int weight_row(int n0, int r, int N) {
 }
 
 template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
-__global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int tiles_n, int tiles_m) {
+__global__ __launch_bounds__((Tile<ACT, GATED, WN, WM, GN, GM>::kLaunch),
+                             (WN * WM <= 4 ? 3 : 2))
+void tile_kernel(Params p, int tiles_n, int tiles_m) {
   using C = Tile<ACT, GATED, WN, WM, GN, GM>;
   constexpr int kSize = OUT == kFp8 ? 1 : 2;
   constexpr int kRow = C::kOut * kSize + 16;  // of the outputs; the odd piece spreads the banks
@@ -539,7 +579,7 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
   auto scales = [&](int u, uint32_t (&v)[C::SU][4]) {
 #pragma unroll
     for (int i = 0; i < C::SU; ++i) {
-      const int r = tid + i * C::kThreads;
+      const int r = tid % C::kScaleThreads + i * C::kScaleThreads;
       if (r >= C::kSRows) break;
       const uint8_t* src;
       if (r < C::TN) {
@@ -549,26 +589,13 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
         const int m = m0 + r - C::TN;
         src = p.a_scale + (int64_t)(m < p.M ? m : p.M - 1) * blocks;
       }
-      if ((u + 1) * 16 <= blocks) {
-        __builtin_memcpy(v[i], src + u * 16, 16);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v[i][j] = 0;
-#pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const int at = u * 16 + j * 4 + k;
-            const uint32_t byte = src[at < blocks ? at : blocks - 1];
-            v[i][j] |= (at < blocks ? byte : 127u) << (8 * k);
-          }
-        }
-      }
+      load_scales(v[i], src, u * 16, blocks);
     }
   };
   auto put_scales = [&](int buf, const uint32_t (&v)[C::SU][4]) {
 #pragma unroll
     for (int i = 0; i < C::SU; ++i) {
-      const int r = tid + i * C::kThreads;
+      const int r = tid % C::kScaleThreads + i * C::kScaleThreads;
       if (r >= C::kSRows) break;
 #pragma unroll
       for (int j = 0; j < 4; ++j) lds_s[(buf * 4 + j) * C::kSRows + r] = v[i][j];
@@ -581,12 +608,38 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
 #pragma unroll
     for (int j = 0; j < WM; ++j) acc[i][j] = {};
 
+  // this workgroup's part of K, in loads of scales and in steps
+  const int u_all = ceil_div(blocks, 16), u_part = ceil_div(u_all, (int)gridDim.y);
+  const int u0 = blockIdx.y * u_part, u1 = u0 + u_part < u_all ? u0 + u_part : u_all;
+  const int t0 = u0 * C::kSteps, t1 = u1 * C::kSteps < steps ? u1 * C::kSteps : steps;
+
   uint32_t sv[C::SU][4];
-  scales(0, sv);
-  put_scales(0, sv);
-  stage(0, 0);
-  if (C::kBufs == 3 && steps > 1) stage(1, 1);
-  __builtin_amdgcn_s_waitcnt(0);
+  if (C::kHelper && wave == GN * GM) {
+    for (int u = u0; u < u1; ++u) {
+      scales(u, sv);
+      put_scales(u & 1, sv);
+      if (u == u0) __syncthreads();
+      // a step's barrier each; those of part u0 follow when u0 + 1 is written
+      const int from = u == u0 ? 0 : (u - 1) * C::kSteps, to = u == u0 ? 0 : u * C::kSteps;
+      for (int t = from; t < to; ++t) __syncthreads();
+    }
+    if (t0 >= t1) __syncthreads();
+    for (int t = (u1 - 1) * C::kSteps; t0 < t1 && t < t1; ++t) __syncthreads();
+    if (gridDim.y == 1) __syncthreads();
+    return;
+  }
+  if (t0 < t1) {
+    if (!C::kHelper) {
+      scales(u0, sv);
+      put_scales(u0 & 1, sv);
+    }
+    stage(t0, 0);
+#pragma unroll
+    for (int i = 1; i < C::kAhead; ++i)
+      if (t0 + i < t1) stage(t0 + i, i);
+  }
+  wait_stages<C::kInFlight, C::kAhead - 1>(t1 - t0 < C::kAhead ? 0 : C::kAhead - 1);
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
   __syncthreads();
 
   // Where a lane reads. Rows 32 apart have one permutation (tokens), so a byte
@@ -597,15 +650,15 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
 #pragma unroll
   for (int i = 0; i < WN; ++i) read_b[i] = spread((b_row + i * 32) * C::WB) ^ (g * 16);
   int buf = 0;
-  for (int t = 0; t < steps; ++t) {
+  for (int t = t0; t < t1; ++t) {
     const int u = t / C::kSteps, s = t % C::kSteps;
-    const bool more = (u + 1) * 16 < blocks;
+    const bool more = u + 1 < u1;
     // Scales are written one step after they were asked for and before this
     // step's loads: what the compiler waits for then is due anyway.
-    if (s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
-    if (s == C::kSteps - 2 && more) scales(u + 1, sv);
+    if (!C::kHelper && s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
+    if (!C::kHelper && s == C::kSteps - 2 && more) scales(u + 1, sv);
     __builtin_amdgcn_sched_barrier(0);
-    if (t + C::kBufs - 1 < steps) stage(t + C::kBufs - 1, buf == 0 ? C::kBufs - 1 : buf - 1);
+    if (t + C::kAhead < t1) stage(t + C::kAhead, buf == 0 ? C::kBufs - 1 : buf - 1);
 
     const uint32_t at_a = read_a + buf * C::kABytes, at_b = buf * C::kBBytes;
     const uint32_t* ls = lds_s + ((u & 1) * 4 + s * 4 / C::kSteps) * C::kSRows;
@@ -711,12 +764,27 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
         }
       }
     }
-    // Until the next step's buffer is full: the loads for the step after it
+    // Until the next step's buffer is full: the loads for the steps after it
     // stay in flight (the last step of a K that it does not divide has none).
-    if (C::kBufs == 3 && (t + 3) * C::KS <= p.K) __builtin_amdgcn_s_waitcnt(wait_code(C::kInFlight, true));
-    else __builtin_amdgcn_s_waitcnt(0);
+    const int last = t + C::kAhead < t1 ? t + C::kAhead : t1 - 1;
+    wait_stages<C::kInFlight, C::kAhead - 1>(last - t - 1 - ((last + 1) * C::KS > p.K));
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __syncthreads();
     buf = buf == C::kBufs - 1 ? 0 : buf + 1;
+  }
+
+  if (gridDim.y > 1) {
+    // as the registers lie: join_kernel reads them so
+    float* to = p.sums + (((int64_t)blockIdx.y * gridDim.x + id) * GN * GM + wave) * WN * WM * 1024;
+#pragma unroll
+    for (int i = 0; i < WN; ++i)
+#pragma unroll
+      for (int j = 0; j < WM; ++j)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          *(float4*)(to + ((i * WM + j) * 4 + r / 4) * 256 + lane * 4) =
+              make_float4(acc[i][j][r], acc[i][j][r + 1], acc[i][j][r + 2], acc[i][j][r + 3]);
+    return;
   }
 
   // Through shared memory, so that a row of the tile leaves in 16-byte pieces.
@@ -799,24 +867,120 @@ __global__ __launch_bounds__(GN * GM * 64, 2) void tile_kernel(Params p, int til
   }
 }
 
+// The parts of K together, in their order: a wave for 32 outputs by 32 tokens.
+template <bool GATED, int OUT, int WN, int WM, int GN, int GM>
+__global__ __launch_bounds__(64) void join_kernel(Params p, int tiles_n, int tiles_m, int parts) {
+  constexpr int H = GATED ? WN / 2 : WN;
+  const int lane = threadIdx.x, lr = lane & 31, g = lane >> 5;
+  int at = blockIdx.x;
+  const int j = at % WM, i = at / WM % H, wave = at / (WM * H) % (GN * GM);
+  const int id = at / (WM * H * GN * GM);
+  const int band = id / (8 * tiles_n), first = band * 8;
+  const int high = tiles_m - first < 8 ? tiles_m - first : 8;
+  const int in_band = id - band * 8 * tiles_n;
+  const int m = (((first + in_band % high) * GM + wave / GN) * WM + j) * 32 + lr;
+  const int n = ((in_band / high * GN + wave % GN) * H + i) * 32 + 4 * g;
+
+  const int64_t part = (int64_t)tiles_n * tiles_m * GN * GM * WN * WM * 1024;
+  const float* from = p.sums + (((int64_t)id * GN * GM + wave) * WN * WM + i * WM + j) * 1024 + lane * 4;
+  float y[16] = {}, u[16] = {};
+#pragma unroll 4
+  for (int s = 0; s < parts; ++s) {
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      const float4 v = *(const float4*)(from + s * part + r / 4 * 256);
+      y[r] += v.x, y[r + 1] += v.y, y[r + 2] += v.z, y[r + 3] += v.w;
+      if constexpr (GATED) {
+        const float4 w = *(const float4*)(from + s * part + H * WM * 1024 + r / 4 * 256);
+        u[r] += w.x, u[r + 1] += w.y, u[r + 2] += w.z, u[r + 3] += w.w;
+      }
+    }
+  }
+  if constexpr (GATED) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) y[r] = activate(p.act, y[r]) * u[r];
+  }
+  if constexpr (OUT == kFp8) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = abs_bits(y[r]) > most ? abs_bits(y[r]) : most;
+    uint32_t a, b;
+    permlane32_pair(most, most, a, b);
+    most = a > b ? a : b;
+    const uint32_t byte = mxfp8_scale_byte(most);
+    const float inv = mx_inverse_scale(byte);
+    if (m < p.M && n < p.N) {
+      uint8_t* o = (uint8_t*)p.out + (int64_t)m * p.ldo + n;
+#pragma unroll
+      for (int r = 0; r < 16; r += 8) {
+        const uint2 q = mxfp8_pack8(y + r, inv, byte == 255u);
+        *(uint32_t*)(o + r * 2) = q.x;
+        *(uint32_t*)(o + r * 2 + 8) = q.y;
+      }
+      if (g == 0) p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
+    }
+  } else if (m < p.M) {
+    using T = typename std::conditional<OUT == kBf16, bf16, fp16>::type;
+    T* o = (T*)p.out + (int64_t)m * p.ldo + n;
+    const bool whole = ((uintptr_t)p.out % 8 | p.ldo % 4) == 0;
+#pragma unroll
+    for (int r = 0; r < 16; r += 4) {
+      union { T v[4]; uint2 q; } t;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) t.v[k] = from_f32<T>(y[r + k]);
+      if (whole && n + 2 * r + 4 <= p.N) {
+        *(uint2*)(o + 2 * r) = t.q;
+      } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (n + 2 * r + k < p.N) o[2 * r + k] = t.v[k];
+      }
+    }
+  }
+}
+
 template <int ACT, bool GATED, int OUT, int WN, int WM, int GN, int GM>
-hipError_t launch_tile(const Params& p, hipStream_t stream) {
+hipError_t launch_tile(const Params& p, int parts, hipStream_t stream) {
   using C = Tile<ACT, GATED, WN, WM, GN, GM>;
   const int64_t tiles_n = ceil_div(p.N, C::kOut), tiles_m = ceil_div(p.M, C::TM);
-  if (tiles_n * tiles_m >= (int64_t)1 << 31) return hipErrorInvalidValue;
+  const int64_t joins = tiles_n * tiles_m * GN * GM * WN * WM / (GATED ? 2 : 1);
+  if (joins >= (int64_t)1 << 31) return hipErrorInvalidValue;
   hipLaunchKernelGGL((tile_kernel<ACT, GATED, OUT, WN, WM, GN, GM>),
-                     dim3((unsigned)(tiles_n * tiles_m)), dim3(C::kThreads), 0, stream, p,
+                     dim3((unsigned)(tiles_n * tiles_m), parts), dim3(C::kLaunch), 0, stream, p,
                      (int)tiles_n, (int)tiles_m);
+  if (parts > 1)
+    hipLaunchKernelGGL((join_kernel<GATED, OUT, WN, WM, GN, GM>), dim3((unsigned)joins), dim3(64), 0,
+                       stream, p, (int)tiles_n, (int)tiles_m, parts);
   return hipGetLastError();
+}
+
+// How many rows a workgroup takes and how many waves share its K. Measured at
+// one bf16 token, us for (tiles of 16 rows, waves, chunks ahead) = (1, 8, 2) /
+// (2, 8, 1) / (2, 4, 1): 4096 x 14336 8.4 / 10.2 / 15.6, 6144 x 4096 5.6 / 5.0 /
+// 6.2, 12288 x 8192 14.7 / 10.9 / 11.4, 32000 x 4096 14.5 / 13.2 / 12.4. Few
+// workgroups need many waves each; many of them hide each other's start, and
+// shared memory that is spent on chunks ahead keeps some of them out.
+template <int ACT, bool GATED, int OUT, int XI>
+hipError_t choose_rows(const Params& p, hipStream_t stream) {
+  if constexpr (OUT == kFp8) {
+    // a block of the output is 32 wide: four tiles
+    return launch_rows<ACT, GATED, OUT, 2, XI, 4, 2>(p, stream);
+  } else {
+    constexpr int RT = GATED ? 1 : 2;
+    const int pairs = ceil_div(p.N, RT * 16);  // workgroups of two tiles
+    if (pairs >= 512) return launch_rows<ACT, GATED, OUT, RT, XI, 4, 1>(p, stream);
+    if constexpr (!GATED)
+      if (pairs < 192) return launch_rows<ACT, GATED, OUT, 1, XI, 8, 2>(p, stream);
+    return launch_rows<ACT, GATED, OUT, RT, XI, 8, 1>(p, stream);
+  }
 }
 
 template <int ACT, bool GATED, int OUT>
 hipError_t launch(const Params& p, hipStream_t stream) {
-  if (p.M > 16) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 1>(p, stream);
-  constexpr int RT = OUT == kFp8 ? 2 : 1;
+  if (p.M > 16) return launch_tile<ACT, GATED, OUT, 2, 4, 4, 1>(p, 1, stream);
   constexpr int kFew = ACT == kFp8 ? 8 : 4;  // tokens in a kilobyte of a chunk
-  if (p.M <= kFew) return launch_rows<ACT, GATED, OUT, RT, 1, 8, GATED ? 3 : 4>(p, stream);
-  return launch_rows<ACT, GATED, OUT, RT, ACT == kFp8 ? 2 : 4, 8, OUT == kFp8 ? 2 : 3>(p, stream);
+  if (p.M <= kFew) return choose_rows<ACT, GATED, OUT, 1>(p, stream);
+  return choose_rows<ACT, GATED, OUT, ACT == kFp8 ? 2 : 4>(p, stream);
 }
 
 template <int ACT>
@@ -846,7 +1010,7 @@ extern "C" hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act
   if (K <= 0 || K % fi::kMxBlock != 0) return hipErrorInvalidValue;
   if (out_type == fi::mx4::kFp8 && N % fi::kMxBlock != 0) return hipErrorInvalidValue;
   fi::mx4::Params p{a, (const uint8_t*)a_scale, (const uint8_t*)b, (const uint8_t*)b_scale,
-                    out, (uint8_t*)out_scale, M, N, K, lda, ldo, act};
+                    out, (uint8_t*)out_scale, M, N, K, lda, ldo, act, nullptr};
   switch (a_type) {
     case 0: return fi::mx4::dispatch<fi::mx4::kBf16>(gated, out_type, p, stream);
     case 1: return fi::mx4::dispatch<fi::mx4::kFp16>(gated, out_type, p, stream);
