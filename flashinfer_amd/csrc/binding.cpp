@@ -94,8 +94,9 @@ hipError_t fi_mx_quant(int dtype, const void* x, void* residual, const void* w, 
                        int aligned, hipStream_t stream);
 hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act, const void* a,
                          const void* a_scale, const void* b, const void* b_scale,
-                         void* out, void* out_scale, int M, int N, int K, int64_t lda,
-                         int64_t ldo, hipStream_t stream);
+                         void* out, void* out_scale, float* floats, int M, int N, int K,
+                         int64_t lda, int64_t ldo, hipStream_t stream);
+int64_t fi_gemm_mxfp4_floats(int gated, int M, int N, int K);
 hipError_t fi_per_group_quant_fp8(int dtype, int trans_scale, const void* x, void* q,
                                   float* scale, int64_t rows, int K, int64_t stride_row,
                                   float eps, hipStream_t stream);
@@ -1116,9 +1117,14 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> mxfp4_product(
   c10::optional<at::Tensor> s;
   if (quantize)
     s = out_scale ? *out_scale : at::empty({M, N / 32}, a.options().dtype(at::kByte));
+  // the sums of the parts of K, where the product is split over it
+  const int64_t floats = fi_gemm_mxfp4_floats(gated, (int)M, (int)N, (int)K);
+  at::Tensor sums;
+  if (floats > 0) sums = at::empty({floats}, a.options().dtype(at::kFloat));
   check_hip(fi_gemm_mxfp4(a_type, out_type, gated, (int)act, a.data_ptr(),
                           as ? as->data_ptr() : nullptr, b.data_ptr(), b_scale.data_ptr(),
-                          o.data_ptr(), s ? s->data_ptr() : nullptr, (int)M, (int)N, (int)K,
+                          o.data_ptr(), s ? s->data_ptr() : nullptr,
+                          floats > 0 ? sums.data_ptr<float>() : nullptr, (int)M, (int)N, (int)K,
                           M > 1 ? a.stride(0) : K, M > 1 ? o.stride(0) : N, cur_stream(a)),
             "fi_gemm_mxfp4");
   return {o, s};

@@ -428,9 +428,15 @@ SHAPES = [(1, 1, 32), (1, 64, 4096), (3, 17, 160), (16, 100, 512), (17, 33, 1056
           (64, 48, 2080), (65, 130, 4096), (130, 301, 544), (257, 513, 1024), (1024, 260, 288)]
 
 
+# one for each tile, with edges on every side: 128 x 32, 64 x 32 and 64 x 64 in
+# parts of K, 64 x 64, 128 x 64, 128 x 128 in two and one parts, 256 x 128
+TILES = [(24, 25000, 64), (20, 100, 9248), (40, 300, 8480), (200, 3100, 288), (33, 20500, 160),
+         (100, 21000, 96), (520, 8450, 96), (1300, 13002, 608)]
+
+
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-@pytest.mark.parametrize("m, n, k", SHAPES)
+@pytest.mark.parametrize("m, n, k", SHAPES + TILES)
 def test_gemm(m, n, k, kind):
     import flashinfer_amd as fi
 
@@ -525,6 +531,67 @@ def test_every_scale_and_special_values(kind):
         out[8] = clean[8]
     out[7] = clean[7]
     assert torch.equal(out, clean), "a NaN row reached another output"
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", [(24, 12512, 64), (20, 64, 9248), (40, 160, 8480), (200, 1568, 288),
+                                     (33, 10272, 160), (100, 10528, 96), (520, 4256, 96),
+                                     (1300, 6528, 608)])
+def test_gated_tiles(m, n, k, kind):
+    import flashinfer_amd as fi
+
+    torch.manual_seed(m * n + k)
+    a, a_scale, a64 = activations(m, k, kind)
+    b, b_scale = weights4(2 * n, k)
+    w64 = from4(b, b_scale)
+    g, u = a64 @ w64[:n].T, a64 @ w64[n:].T
+    og, ou = product_off(a64, w64[:n], kind), product_off(a64, w64[n:], kind)
+    want = act64(g, "silu") * u
+    og = 1.13 * og + 8 * 2.0 ** -24 * g.abs()
+    off = og * (u.abs() + ou) + act64(g, "silu").abs() * ou
+    out = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=torch.bfloat16)
+    err, bound = (out.double() - want).abs(), off + 2.0 ** -8 * (want.abs() + off)
+    assert (err <= bound).all(), f"off by {(err / bound).max()} of the bound"
+    q, s = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=FP8)
+    check8(q, s, want, off)
+
+
+@gpu
+@pytest.mark.parametrize("m, n, k", [(3, 40, 160), (24, 12500, 64), (40, 300, 8480), (200, 3100, 288),
+                                     (100, 10500, 96), (520, 8450, 96), (1300, 13002, 96)])
+def test_fp16_with_weights_outside_its_range(m, n, k):
+    """Blocks whose weights fp16 does not hold, some of a tile and some tiles:
+    the results are as exact as elsewhere, and the other tiles' too."""
+    import flashinfer_amd as fi
+
+    torch.manual_seed(m)
+    a, _, a64 = activations(m, k, "fp16")
+    b, b_scale = weights4(n, k)
+    b_scale[n // 3, 0], b_scale[n // 3, -1] = 103, 98  # below 2^-23, and far below
+    b_scale[-1, -1] = 141                              # 6 * 2^14 is no fp16
+    a[m // 2, :32] = 0
+    a64 = a.double()
+    w64 = from4(b, b_scale)
+    want, off = a64 @ w64.T, product_off(a64, w64, "fp16")
+    out = fi.gemm_mxfp4_nt(a, b, b_scale, out_dtype=torch.bfloat16)
+    err, bound = (out.double() - want).abs(), off + 2.0 ** -8 * (want.abs() + off)
+    assert (err <= bound).all(), f"off by {(err / bound).max()} of the bound"
+
+
+@gpu
+def test_rows_too_far_apart_for_32_bits():
+    """A tile counts bytes in 32 bits; rows 16 MB apart do not fit it."""
+    import flashinfer_amd as fi
+
+    torch.manual_seed(0)
+    m, n, k = 40, 96, 256
+    wide = torch.zeros(m, (1 << 23) + 8, dtype=torch.bfloat16, device="cuda")
+    wide[:, :k] = torch.randn(m, k, device="cuda")
+    b, b_scale = weights4(n, k)
+    want = fi.gemm_mxfp4_nt(wide[:, :k].contiguous(), b, b_scale)
+    got = fi.gemm_mxfp4_nt(wide[:, :k], b, b_scale)
+    torch.testing.assert_close(got, want, rtol=2.0 ** -7, atol=1e-3)
 
 
 @gpu
