@@ -3,6 +3,7 @@
 // launchers (fast incremental builds: kernel TUs compile in seconds).
 #include <torch/extension.h>
 
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime.h>
 
@@ -938,6 +939,11 @@ bool is_scale(const at::Tensor& t) {
   return t.scalar_type() == at::kByte || t.scalar_type() == at::kFloat8_e8m0fnu;
 }
 
+// at::empty without the dispatcher: 0.3 us less of a call that takes five
+at::Tensor empty_like_on(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
+  return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), c10::nullopt));
+}
+
 bool on_16(const at::Tensor& t) {
   return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
 }
@@ -1004,8 +1010,8 @@ std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tens
   if (out_scale) refuse_overlap(name, *out_scale, {&x, r, wp, out ? &*out : nullptr});
 
   c10::DeviceGuard guard(x.device());
-  at::Tensor q = out ? *out : at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
-  at::Tensor s = out_scale ? *out_scale : at::empty(scale_shape, x.options().dtype(at::kByte));
+  at::Tensor q = out ? *out : empty_like_on(x, x.sizes(), at::kFloat8_e4m3fn);
+  at::Tensor s = out_scale ? *out_scale : empty_like_on(x, scale_shape, at::kByte);
   const int64_t step = 16 / x.element_size();
   const bool aligned = on_16(x) && (rows <= 1 || sx % step == 0) &&
                        (!r || (on_16(*r) && (rows <= 1 || sr % step == 0))) &&
@@ -1113,14 +1119,14 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> mxfp4_product(
   }
 
   c10::DeviceGuard guard(a.device());
-  at::Tensor o = out ? *out : at::empty({M, N}, a.options().dtype(type));
+  at::Tensor o = out ? *out : empty_like_on(a, {M, N}, type);
   c10::optional<at::Tensor> s;
   if (quantize)
-    s = out_scale ? *out_scale : at::empty({M, N / 32}, a.options().dtype(at::kByte));
+    s = out_scale ? *out_scale : empty_like_on(a, {M, N / 32}, at::kByte);
   // the sums of the parts of K, where the product is split over it
   const int64_t floats = fi_gemm_mxfp4_floats(gated, (int)M, (int)N, (int)K);
   at::Tensor sums;
-  if (floats > 0) sums = at::empty({floats}, a.options().dtype(at::kFloat));
+  if (floats > 0) sums = empty_like_on(a, {floats}, at::kFloat);
   check_hip(fi_gemm_mxfp4(a_type, out_type, gated, (int)act, a.data_ptr(),
                           as ? as->data_ptr() : nullptr, b.data_ptr(), b_scale.data_ptr(),
                           o.data_ptr(), s ? s->data_ptr() : nullptr,

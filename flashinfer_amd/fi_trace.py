@@ -9,6 +9,8 @@ import json
 import os
 from pathlib import Path
 
+from . import trace_apply as _ta
+
 _DIR = os.environ.get("FLASHINFER_TRACE_DUMP", "")
 _seen = set()
 
@@ -29,9 +31,7 @@ def fi_trace(fn):
     @functools.wraps(fn)
     def wrapper(*args, **kwargs):
         # trace_apply hook: a registered substitute takes over this call
-        from . import trace_apply as _ta
-
-        sub = _ta._dispatch(fn.__name__) if _ta.is_enabled() else None
+        sub = _ta._dispatch(fn.__name__) if _ta._enabled else None
         if sub is not None:
             return sub(*args, **kwargs)
         if _DIR:
