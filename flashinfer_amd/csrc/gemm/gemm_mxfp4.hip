@@ -5,43 +5,63 @@
 namespace fi {
 namespace mx4 {
 
-// The largest tile that still gives the chip's 256 CUs something to do: tokens
-// are read once for each tile of weight rows and weights once for each tile of
-// tokens, so large tiles move less. Measured (us, K = 4096 unless said) where
-// two of them meet, in the order of the enum:
-//   8-bit tokens 4096 x 6144: 256x128 93, 128x128 104; 1024 x 6144: 39 and 32
-//   bf16 1024 x 4096: 128x128 43, 128x128x2 37, 128x64x2 48
-//   8-bit 512 x 4096, K = 14336: 128x128x2 43, 128x64x2 41, 64x64x4 53
-//   bf16 128 x 4096: 64x64x4 14.4, 64x32x4 11.5; 256 x 4096: 15.7 and 20.9
-//   bf16 24 x 28672: 128x32x4 16.0, 64x32x4 21.2, 128x64x2 23.4
-// With a long K and few tiles K is split over workgroups too, and a second
-// kernel joins the parts: 8-bit 64 x 4096, K = 14336, 64x64x4 in 1 / 2 / 4
-// parts 27 / 18.9 / 14.7.
-Plan make_plan(int M, int N, int K, bool gated) {
+// What a tile costs: us to start and to finish, and us for 1024 of K where a CU
+// holds one workgroup and where it holds two. Measured with K = 1024 and 4096 at
+// 256 and 512 tiles: large tiles move fewer bytes for a product, small ones
+// leave fewer CUs without work.
+struct Cost {
+  int shape, rows, tokens;
+  float start, one, two;  // two: 0 where a CU has room for one
+};
+constexpr Cost kCosts16[] = {
+    {k256x128, 256, 128, 4.2f, 14.0f, 25.8f}, {k128x128, 128, 128, 3.0f, 8.9f, 14.3f},
+    {k128x128x2, 128, 128, 3.5f, 7.1f, 0.f},  {k128x64x2, 128, 64, 1.7f, 4.9f, 0.f},
+    {k64x64x4, 64, 64, 0.8f, 2.8f, 0.f},      {k64x32x4, 64, 32, 0.6f, 1.9f, 0.f},
+    {k128x32x4, 128, 32, 1.2f, 2.8f, 0.f},
+};
+constexpr Cost kCosts8[] = {
+    {k256x128, 256, 128, 4.6f, 8.4f, 13.2f}, {k128x128, 128, 128, 2.4f, 5.7f, 7.2f},
+    {k128x128x2, 128, 128, 2.9f, 3.9f, 0.f}, {k128x64x2, 128, 64, 1.1f, 2.7f, 0.f},
+    {k64x64x4, 64, 64, 0.7f, 1.9f, 0.f},     {k64x32x4, 64, 32, 0.4f, 1.6f, 0.f},
+    {k128x32x4, 128, 32, 0.7f, 2.1f, 0.f},
+};
+
+// The kernel and tile of the least cost, and in how many parts of K the tiles
+// are computed. Parts cost a second kernel (3 us) and the way of their sums
+// through memory.
+Plan make_plan(int M, int N, int K, bool gated, bool act8) {
   if (M <= 16) return {kRows, 1, 0};
+  constexpr int kCus = kNumCU, kMostParts = 16;
   const int64_t rows = gated ? 2 * (int64_t)N : N;
-  auto tiles = [&](int r, int t) { return ceil_div64(rows, r) * ceil_div64(M, t); };
-  if (M > 32 && tiles(256, 128) >= 512) return {k256x128, 1, 0};
-  if (M > 64 && tiles(128, 128) > 256) return {k128x128, 1, 0};
-  if (M <= 32 && tiles(128, 32) >= 192) return {k128x32x4, 1, 0};
-  if (M > 64 && tiles(128, 128) >= 160) return {k128x128x2, 1, 0};
-  if (M > 32 && tiles(128, 64) >= 160) return {k128x64x2, 1, 0};
-  if (M > 32 && tiles(64, 64) >= 192) return {k64x64x4, 1, 0};
   const int loads = ceil_div(K, 512);  // of scales; a part holds whole ones
-  if (loads < 16) return {k64x32x4, 1, 0};
-  const int wide = M > 32 ? 64 : 32;
-  int64_t parts = 256 / tiles(64, wide);
-  if (parts > loads / 6) parts = loads / 6;
-  if (parts <= 1) return {M > 32 ? k64x64x4 : k64x32x4, 1, 0};
-  return {M > 32 ? k64x64x4 : k64x32x4, (int)parts, parts * tiles(64, wide) * 64 * wide};
+  Plan best{kRows, 1, 0};
+  float least = 0.f;
+  for (int i = 0; i < 7; ++i) {
+    const Cost& c = act8 ? kCosts8[i] : kCosts16[i];
+    const int64_t tiles = ceil_div64(rows, c.rows) * ceil_div64(M, c.tokens);
+    for (int parts = 1; parts <= kMostParts && parts <= loads; ++parts) {
+      if (parts > 1 && tiles * parts > 2 * kCus) break;
+      const float k = parts > 1 ? 0.5f * ceil_div(loads, parts) : K / 1024.f;
+      const int64_t each = ceil_div64(tiles * parts, kCus);  // workgroups of a CU
+      float us = c.two > 0.f ? each / 2 * (c.start + c.two * k) + each % 2 * (c.start + c.one * k)
+                             : each * (c.start + c.one * k);
+      const int64_t floats = parts > 1 ? parts * tiles * c.rows * c.tokens : 0;
+      if (parts > 1) us += 3.f + floats * 8 / 3e6f;
+      if (best.shape == kRows || us < least) {
+        least = us;
+        best = {c.shape, parts, floats};
+      }
+    }
+  }
+  return best;
 }
 
 }  // namespace mx4
 }  // namespace fi
 
 // How many floats of workspace fi_gemm_mxfp4 wants for this product.
-extern "C" int64_t fi_gemm_mxfp4_floats(int gated, int M, int N, int K) {
-  return M > 0 && N > 0 ? fi::mx4::make_plan(M, N, K, gated).floats : 0;
+extern "C" int64_t fi_gemm_mxfp4_floats(int a_type, int gated, int M, int N, int K) {
+  return M > 0 && N > 0 ? fi::mx4::make_plan(M, N, K, gated, a_type == fi::mx4::kFp8).floats : 0;
 }
 
 // a_type: 0 bf16, 1 fp16, 2 e4m3 with scale bytes; out_type the same, 2 for the
@@ -70,7 +90,7 @@ extern "C" hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act
     }
     return hipErrorInvalidValue;
   };
-  const Plan plan = make_plan(M, N, K, gated);
+  const Plan plan = make_plan(M, N, K, gated, a_type == kFp8);
   if (plan.parts > 1 && !floats) return hipErrorInvalidValue;
   const int a_size = a_type == kFp8 ? 1 : 2, out_size = out_type == kFp8 ? 1 : 2;
   // A tile counts its bytes in 32 bits. Rows further apart than that allows go

@@ -62,13 +62,33 @@ __device__ __forceinline__ float times_logistic(float g, float t) {
   return g * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(t));
 }
 
+// erfc(x) within 1.2e-7 of its value, the rounding of the exponent apart: the
+// Chebyshev fit of W. H. Press et al., Numerical Recipes (2nd ed., 6.2), where
+// erfc(z) = t exp(-z^2 + P(t)), t = 1 / (1 + z / 2), z = |x|. It keeps the small
+// negative tail of the activation, which 1 + erf rounds away.
+__device__ __forceinline__ float erfc_close(float x) {
+  const float z = __builtin_fabsf(x);
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.5f * z);
+  float q = 0.17087277f;
+  q = q * t - 0.82215223f;
+  q = q * t + 1.48851587f;
+  q = q * t - 1.13520398f;
+  q = q * t + 0.27886807f;
+  q = q * t - 0.18628806f;
+  q = q * t + 0.09678418f;
+  q = q * t + 0.37409196f;
+  q = q * t + 1.00002368f;
+  q = q * t - 1.26551223f;
+  const float r = t * __builtin_amdgcn_exp2f((q - z * z) * 1.4426950408889634f);
+  return x < 0.f ? 2.f - r : r;
+}
+
 template <int kAct>
 __device__ __forceinline__ float activate(float g) {
   if constexpr (kAct == 0) {
     return times_logistic(g, g * -1.4426950408889634f);
   } else if constexpr (kAct == 1) {
-    // erfc keeps the small negative tail that 1 + erf rounds away
-    return 0.5f * g * erfcf(g * -0.70710678118654752f);
+    return 0.5f * g * erfc_close(g * -0.70710678118654752f);
   } else {
     // 0.5 (1 + tanh(u)) = 1 / (1 + exp(-2u)), u = sqrt(2 / pi) (g + 0.044715 g^3)
     return times_logistic(g, g * (-2.3022081985f - 0.1029432397f * g * g));
@@ -395,26 +415,28 @@ void rows_kernel(Params p) {
     *(floatx4*)(join + (wave * 16 + lr) * C::LD + t * 16 + g * 4) = acc[t];
   __syncthreads();
 
-  // eight neighbouring outputs of one token to a thread
-  constexpr int G8 = RT * 2;
-  for (int i = tid; i < 16 * G8; i += WAVES * 64) {
-    const int m = i / G8, nl = (i % G8) * 8, n = n0 + nl;
-    float y[8];
+  auto joined = [&](int m, int nl) {
+    float s = 0.f, u = 0.f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      float s = 0.f, u = 0.f;
-#pragma unroll
-      for (int w = 0; w < WAVES; ++w) {
-        s += join[(w * 16 + m) * C::LD + nl + j];
-        if constexpr (GATED) u += join[(w * 16 + m) * C::LD + RT * 16 + nl + j];
-      }
-      y[j] = GATED ? activate(p.act, s) * u : s;
+    for (int w = 0; w < WAVES; ++w) {
+      s += join[(w * 16 + m) * C::LD + nl];
+      if constexpr (GATED) u += join[(w * 16 + m) * C::LD + RT * 16 + nl];
     }
-    if constexpr (OUT8) {
-      // N is a multiple of 32 here and a quad holds one block
+    return GATED ? activate(p.act, s) * u : s;
+  };
+  if constexpr (OUT8) {
+    // Eight neighbouring outputs of one token to a thread: a quad holds one
+    // block. N is a multiple of 32 here.
+    constexpr int G8 = RT * 2;
+    for (int i = tid; i < 16 * G8; i += WAVES * 64) {
+      const int m = i / G8, nl = (i % G8) * 8, n = n0 + nl;
+      float y[8];
       uint32_t most = 0;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) most = abs_bits(y[j]) > most ? abs_bits(y[j]) : most;
+      for (int j = 0; j < 8; ++j) {
+        y[j] = joined(m, nl + j);
+        most = abs_bits(y[j]) > most ? abs_bits(y[j]) : most;
+      }
       most = quad_max(most);
       const uint32_t byte = mxfp8_scale_byte(most);
       if (m < p.M && n < p.N) {
@@ -423,11 +445,12 @@ void rows_kernel(Params p) {
         if (nl % 32 == 0)
           p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
       }
-    } else if (m < p.M) {
-      uint16_t* o = (uint16_t*)p.out + (int64_t)m * p.ldo + n;
-#pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (n + j < p.N) o[j] = to16(y[j], p.out_fp16);
+    }
+  } else {
+    for (int i = tid; i < 16 * RT * 16; i += WAVES * 64) {
+      const int m = i / (RT * 16), nl = i % (RT * 16), n = n0 + nl;
+      if (m < p.M && n < p.N)
+        ((uint16_t*)p.out)[(int64_t)m * p.ldo + n] = to16(joined(m, nl), p.out_fp16);
     }
   }
 }
@@ -472,7 +495,7 @@ struct Tile {
   static constexpr int kStage = kABytes + kBBytes, kScales = 2 * 16 * kSRows;
   // a workgroup of four waves shares a CU with another
   static constexpr int kMost = kThreads <= 256 ? kLdsBytes / 2 : kLdsBytes;
-  static constexpr int kFit = (kMost - kScales - 16) / (kStage * GK);
+  static constexpr int kFit = (kMost - kScales - (ACT == kFp16 ? 16 : 0)) / (kStage * GK);
   static constexpr int kBufs = kFit < 6 ? kFit : 6;
   static constexpr int kAhead = kBufs - 1;               // steps on their way
   static constexpr int kRing = GK * kBufs * kStage;
@@ -627,26 +650,27 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
   uint32_t sv[C::SU][4];
   // What the helping wave does during a pass. Barriers as the others have
   // them: one ahead of the rounds and one a round. During load u of the scales
-  // it writes load u + 1, which it asked for during load u - 1.
+  // it writes load u + 1 and asks for load u + 4: every eighth load of a row
+  // meets a new line of memory, which takes longer than the rounds of one load.
   auto bring_scales = [&]() {
-    constexpr int kRounds = C::kSteps / GK;
-    uint32_t next[C::SU][4];
-    if (u0 < u1) {
-      scales(u0, sv);
-      if (u0 + 1 < u1) scales(u0 + 1, next);
-      put_scales(u0 & 1, sv);
-    }
+    constexpr int kRounds = C::kSteps / GK, kSets = 4;
+    uint32_t set[kSets][C::SU][4];
+#pragma unroll
+    for (int i = 0; i < kSets; ++i)
+      if (u0 + i < u1) scales(u0 + i, set[i]);
+    if (u0 < u1) put_scales(u0 & 1, set[0]);
     __syncthreads();
-    auto during = [&](int u, uint32_t (&far)[C::SU][4], uint32_t (&near)[C::SU][4]) {
-      if (u + 2 < u1) scales(u + 2, far);
-      const int to = u + 1 < u1 ? kRounds : rounds - (u - u0) * kRounds;
-      for (int r = 1; r < to; ++r) __syncthreads();
-      if (u + 1 < u1) put_scales((u + 1) & 1, near);
-      __syncthreads();
-    };
-    for (int u = u0; u < u1; u += 2) {
-      during(u, sv, next);
-      if (u + 1 < u1) during(u + 1, next, sv);
+    for (int first = u0; first < u1; first += kSets) {
+#pragma unroll
+      for (int i = 0; i < kSets; ++i) {
+        const int u = first + i;
+        if (u >= u1) break;
+        if (u + kSets < u1) scales(u + kSets, set[i]);
+        const int to = u + 1 < u1 ? kRounds : rounds - (u - u0) * kRounds;
+        for (int r = 1; r < to; ++r) __syncthreads();
+        if (u + 1 < u1) put_scales((u + 1) & 1, set[(i + 1) % kSets]);
+        __syncthreads();
+      }
     }
   };
 
@@ -684,10 +708,10 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
       const int t = first_t + round * GK;
       const int u = t / C::kSteps, s = t % C::kSteps;
       const bool more = u + 1 < u1;
-      // Scales are written one step after they were asked for and before this
-      // step's loads: what the compiler waits for then is due anyway.
+      // Scales are written before the loads of a step: what the compiler waits
+      // for then is due at this step's end anyway.
       if (!C::kHelper && s == C::kSteps - 1 && more) put_scales((u + 1) & 1, sv);
-      if (!C::kHelper && s == C::kSteps - 2 && more) scales(u + 1, sv);
+      if (!C::kHelper && s == 0 && more) scales(u + 1, sv);
       __builtin_amdgcn_sched_barrier(0);
       if (t + C::kAhead * GK < t1)
         stage(t + C::kAhead * GK, buf == 0 ? C::kBufs - 1 : buf - 1);
@@ -925,23 +949,28 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
   }
   __syncthreads();
   constexpr int kPieces = C::kOut * kSize / 16, kEach = 16 / kSize;
-  const bool whole = ((uintptr_t)p.out % 16 | p.ldo * kSize % 16) == 0;
-  for (int i = tid; i < C::TM * kPieces; i += C::kThreads) {
-    const int ml = i / kPieces, nl = i % kPieces * kEach;
-    const int m = m0 + ml, n = n0 + nl;
-    if (m >= p.M || n >= p.N) continue;
-    const uint8_t* from = lds + ml * kRow + nl * kSize;
-    uint8_t* to = (uint8_t*)p.out + ((int64_t)m * p.ldo + n) * kSize;
-    if (whole && n + kEach <= p.N) {
-      *(uint4*)to = *(const uint4*)from;
-    } else if constexpr (OUT8) {
-      // rows at multiples of 8, N at one of 32
-      ((uint2*)to)[0] = ((const uint2*)from)[0];
-      ((uint2*)to)[1] = ((const uint2*)from)[1];
-    } else {
-#pragma unroll
-      for (int k = 0; k < kEach; ++k)
-        if (n + k < p.N) ((uint16_t*)to)[k] = ((const uint16_t*)from)[k];
+  const bool whole = OUT8 ? ((uintptr_t)p.out % 16 | p.ldo % 16) == 0
+                          : ((uintptr_t)p.out % 16 | p.ldo % 8 | p.N % 8) == 0;
+  if (OUT8 || whole) {
+    for (int i = tid; i < C::TM * kPieces; i += C::kThreads) {
+      const int ml = i / kPieces, nl = i % kPieces * kEach;
+      const int m = m0 + ml, n = n0 + nl;
+      if (m >= p.M || n >= p.N) continue;
+      const uint8_t* from = lds + ml * kRow + nl * kSize;
+      uint8_t* to = (uint8_t*)p.out + ((int64_t)m * p.ldo + n) * kSize;
+      if (whole) {
+        *(uint4*)to = *(const uint4*)from;
+      } else {  // MXFP8: rows at multiples of 8, N at one of 32
+        ((uint2*)to)[0] = ((const uint2*)from)[0];
+        ((uint2*)to)[1] = ((const uint2*)from)[1];
+      }
+    }
+  } else {
+    // odd rows: one output a lane, so that a wave still writes 128 bytes in a row
+    for (int i = tid; i < C::TM * C::kOut; i += C::kThreads) {
+      const int ml = i / C::kOut, nl = i % C::kOut, m = m0 + ml, n = n0 + nl;
+      if (m < p.M && n < p.N)
+        ((uint16_t*)p.out)[(int64_t)m * p.ldo + n] = *(const uint16_t*)(lds + ml * kRow + nl * 2);
     }
   }
 }
@@ -1056,18 +1085,20 @@ struct Plan {
 // (2, 8, 1) / (2, 4, 1): 4096 x 14336 8.4 / 10.2 / 15.6, 6144 x 4096 5.6 / 5.0 /
 // 6.2, 12288 x 8192 14.7 / 10.9 / 11.4, 32000 x 4096 14.5 / 13.2 / 12.4. Few
 // workgroups need many waves each; many of them hide each other's start, and
-// shared memory that is spent on chunks ahead keeps some of them out.
+// shared memory that is spent on chunks ahead keeps some of them out. Four
+// tiles with an MXFP8 output, (2, 8, 1) / (2, 4, 2): 4096 x 4096 7.6 / 8.2,
+// 14336 x 4096 13.2 / 12.4. Sixteen waves lose everywhere (6144 x 4096 10.2).
 template <int ACT, bool GATED, bool OUT8, int XI>
 hipError_t choose_rows(const Params& p, hipStream_t stream) {
   if constexpr (OUT8) {
     // a block of the output is 32 wide: four tiles
+    if (p.N < 384 * 32) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 1>(p, stream);
     return launch_rows<ACT, GATED, OUT8, 2, XI, 4, 2>(p, stream);
   } else {
     constexpr int RT = GATED ? 1 : 2;
     const int pairs = ceil_div(p.N, RT * 16);  // workgroups of two tiles
     if (pairs >= 512) return launch_rows<ACT, GATED, OUT8, RT, XI, 4, 1>(p, stream);
-    if constexpr (!GATED)
-      if (pairs < 192) return launch_rows<ACT, GATED, OUT8, 1, XI, 8, 2>(p, stream);
+    if (pairs < 192) return launch_rows<ACT, GATED, OUT8, 1, XI, 8, 2>(p, stream);
     return launch_rows<ACT, GATED, OUT8, RT, XI, 8, 1>(p, stream);
   }
 }
