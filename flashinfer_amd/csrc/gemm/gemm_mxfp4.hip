@@ -6,24 +6,27 @@ namespace fi {
 namespace mx4 {
 
 // What a tile costs: us to start and to finish, and us for 1024 of K where a CU
-// holds one workgroup and where it holds two. Measured with K = 1024 and 4096 at
-// 256 and 512 tiles: large tiles move fewer bytes for a product, small ones
-// leave fewer CUs without work.
+// holds one workgroup and where it holds two. Fitted to K = 1024, 2048 and 7680
+// with 256, 512 and 1024 tiles (each time within 17 %; 25 % for 128 x 32). Large
+// tiles move fewer bytes for a product, small ones leave fewer CUs without work.
+// `apart`: how much longer it takes where rows of a do not start at multiples of
+// 128 bytes, so that every piece of one lies in two lines (K = 7520 to 7680).
 struct Cost {
   int shape, rows, tokens;
   float start, one, two;  // two: 0 where a CU has room for one
+  float apart;
 };
 constexpr Cost kCosts16[] = {
-    {k256x128, 256, 128, 4.2f, 14.0f, 25.8f}, {k128x128, 128, 128, 3.0f, 8.9f, 14.3f},
-    {k128x128x2, 128, 128, 3.5f, 7.1f, 0.f},  {k128x64x2, 128, 64, 1.7f, 4.9f, 0.f},
-    {k64x64x4, 64, 64, 0.8f, 2.8f, 0.f},      {k64x32x4, 64, 32, 0.6f, 1.9f, 0.f},
-    {k128x32x4, 128, 32, 1.2f, 2.8f, 0.f},
+    {k256x128, 256, 128, 4.1f, 14.3f, 26.8f, 1.07f}, {k128x128, 128, 128, 2.6f, 8.8f, 14.9f, 1.05f},
+    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.07f},  {k128x64x2, 128, 64, 2.6f, 4.9f, 0.f, 1.06f},
+    {k64x64x4, 64, 64, 1.9f, 2.6f, 0.f, 1.13f},      {k64x32x4, 64, 32, 1.4f, 1.8f, 0.f, 1.15f},
+    {k128x32x4, 128, 32, 1.9f, 2.9f, 0.f, 1.1f},
 };
 constexpr Cost kCosts8[] = {
-    {k256x128, 256, 128, 4.6f, 8.4f, 13.2f}, {k128x128, 128, 128, 2.4f, 5.7f, 7.2f},
-    {k128x128x2, 128, 128, 2.9f, 3.9f, 0.f}, {k128x64x2, 128, 64, 1.1f, 2.7f, 0.f},
-    {k64x64x4, 64, 64, 0.7f, 1.9f, 0.f},     {k64x32x4, 64, 32, 0.4f, 1.6f, 0.f},
-    {k128x32x4, 128, 32, 0.7f, 2.1f, 0.f},
+    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.22f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.11f},
+    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.26f}, {k128x64x2, 128, 64, 1.9f, 2.7f, 0.f, 1.41f},
+    {k64x64x4, 64, 64, 1.7f, 1.7f, 0.f, 1.21f},     {k64x32x4, 64, 32, 0.8f, 1.5f, 0.f, 1.13f},
+    {k128x32x4, 128, 32, 1.3f, 2.2f, 0.f, 1.26f},
 };
 
 // The kernel and tile of the least cost, and in how many parts of K the tiles
@@ -34,6 +37,7 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8) {
   constexpr int kCus = kNumCU, kMostParts = 16;
   const int64_t rows = gated ? 2 * (int64_t)N : N;
   const int loads = ceil_div(K, 512);  // of scales; a part holds whole ones
+  const bool odd = K % (act8 ? 128 : 64) != 0;
   Plan best{kRows, 1, 0};
   float least = 0.f;
   for (int i = 0; i < 7; ++i) {
@@ -41,7 +45,7 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8) {
     const int64_t tiles = ceil_div64(rows, c.rows) * ceil_div64(M, c.tokens);
     for (int parts = 1; parts <= kMostParts && parts <= loads; ++parts) {
       if (parts > 1 && tiles * parts > 2 * kCus) break;
-      const float k = parts > 1 ? 0.5f * ceil_div(loads, parts) : K / 1024.f;
+      const float k = (parts > 1 ? 0.5f * ceil_div(loads, parts) : K / 1024.f) * (odd ? c.apart : 1.f);
       const int64_t each = ceil_div64(tiles * parts, kCus);  // workgroups of a CU
       float us = c.two > 0.f ? each / 2 * (c.start + c.two * k) + each % 2 * (c.start + c.one * k)
                              : each * (c.start + c.one * k);

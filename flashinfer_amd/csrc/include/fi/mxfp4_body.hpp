@@ -975,12 +975,15 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
   }
 }
 
-// The parts of K together, in their order: a wave for 32 outputs by 32 tokens.
+// The parts of K together: a workgroup for 32 outputs by 32 tokens. Each of its
+// waves sums a quarter of the parts, the quarters follow in their order.
 template <bool GATED, bool OUT8, int WN, int WM, int GN, int GM, int GK>
-__global__ __launch_bounds__(64) void join_kernel(Params p, int tiles_n, int tiles_m, int parts) {
-  constexpr int H = GATED ? WN / 2 : WN;
-  const int lane = threadIdx.x, lr = lane & 31, g = lane >> 5;
-  int at = blockIdx.x;
+__global__ __launch_bounds__(256) void join_kernel(Params p, int tiles_n, int tiles_m, int parts) {
+  constexpr int H = GATED ? WN / 2 : WN, kSums = GATED ? 32 : 16;
+  __shared__ float quarter[3][kSums][64];
+  const int lane = threadIdx.x & 63, lr = lane & 31, g = lane >> 5;
+  const int q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int at = blockIdx.x;
   const int j = at % WM, i = at / WM % H, wave = at / (WM * H) % (GN * GM);
   const int id = at / (WM * H * GN * GM);
   const int band = id / (8 * tiles_n), first = band * 8;
@@ -991,23 +994,30 @@ __global__ __launch_bounds__(64) void join_kernel(Params p, int tiles_n, int til
 
   const int64_t part = (int64_t)tiles_n * tiles_m * GN * GM * WN * WM * 1024;
   const float* from = p.sums + (((int64_t)id * GN * GM + wave) * WN * WM + i * WM + j) * 1024 + lane * 4;
-  float y[16] = {}, u[16] = {};
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
+  float sum[kSums] = {};  // of the gate, then of up
+  const int each = ceil_div(parts, 4);
+  const int s1 = (q + 1) * each < parts ? (q + 1) * each : parts;
+#pragma unroll 2
+  for (int s = q * each; s < s1; ++s) {
 #pragma unroll
-    for (int r = 0; r < 16; r += 4) {
-      const float4 v = *(const float4*)(from + s * part + r / 4 * 256);
-      y[r] += v.x, y[r + 1] += v.y, y[r + 2] += v.z, y[r + 3] += v.w;
-      if constexpr (GATED) {
-        const float4 w = *(const float4*)(from + s * part + H * WM * 1024 + r / 4 * 256);
-        u[r] += w.x, u[r + 1] += w.y, u[r + 2] += w.z, u[r + 3] += w.w;
-      }
+    for (int r = 0; r < kSums; r += 4) {
+      const float4 v = *(const float4*)(from + s * part + r / 16 * H * WM * 1024 + r % 16 / 4 * 256);
+      sum[r] += v.x, sum[r + 1] += v.y, sum[r + 2] += v.z, sum[r + 3] += v.w;
     }
   }
-  if constexpr (GATED) {
+  if (q > 0) {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) y[r] = activate(p.act, y[r]) * u[r];
+    for (int r = 0; r < kSums; ++r) quarter[q - 1][r][lane] = sum[r];
   }
+  __syncthreads();
+  if (q > 0) return;
+#pragma unroll
+  for (int k = 0; k < 3; ++k)
+#pragma unroll
+    for (int r = 0; r < kSums; ++r) sum[r] += quarter[k][r][lane];
+  float y[16];
+#pragma unroll
+  for (int r = 0; r < 16; ++r) y[r] = GATED ? activate(p.act, sum[r]) * sum[r + kSums - 16] : sum[r];
   if constexpr (OUT8) {
     uint32_t most = 0;
 #pragma unroll
@@ -1056,7 +1066,7 @@ hipError_t launch_tile(const Params& p, int parts, hipStream_t stream) {
                      dim3((unsigned)(tiles_n * tiles_m), parts), dim3(C::kLaunch), 0, stream, p,
                      (int)tiles_n, (int)tiles_m);
   if (parts > 1)
-    hipLaunchKernelGGL((join_kernel<GATED, OUT8, WN, WM, GN, GM, GK>), dim3((unsigned)joins), dim3(64), 0,
+    hipLaunchKernelGGL((join_kernel<GATED, OUT8, WN, WM, GN, GM, GK>), dim3((unsigned)joins), dim3(256), 0,
                        stream, p, (int)tiles_n, (int)tiles_m, parts);
   return hipGetLastError();
 }
