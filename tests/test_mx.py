@@ -434,9 +434,14 @@ TILES = [(24, 25000, 64), (20, 100, 9248), (40, 300, 8480), (200, 3100, 288), (3
          (100, 21000, 96), (520, 8450, 96), (1300, 13002, 608)]
 
 
+# the kernel for few tokens: K in one, two and three slabs of scales, and the
+# three ways to share it
+FEW = [(1, 70, 12320), (5, 40, 6176), (16, 33, 14336), (3, 16500, 6240), (2, 7001, 96), (9, 7000, 6144)]
+
+
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-@pytest.mark.parametrize("m, n, k", SHAPES + TILES)
+@pytest.mark.parametrize("m, n, k", SHAPES + TILES + FEW)
 def test_gemm(m, n, k, kind):
     import flashinfer_amd as fi
 
@@ -537,7 +542,8 @@ def test_every_scale_and_special_values(kind):
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
 @pytest.mark.parametrize("m, n, k", [(24, 12512, 64), (20, 64, 9248), (40, 160, 8480), (200, 1568, 288),
                                      (33, 10272, 160), (100, 10528, 96), (520, 4256, 96),
-                                     (1300, 6528, 608)])
+                                     (1300, 6528, 608), (1, 64, 12320), (16, 32, 6176), (5, 12320, 160),
+                                     (3, 16512, 96)])
 def test_gated_tiles(m, n, k, kind):
     import flashinfer_amd as fi
 
@@ -577,6 +583,37 @@ def test_fp16_with_weights_outside_its_range(m, n, k):
     out = fi.gemm_mxfp4_nt(a, b, b_scale, out_dtype=torch.bfloat16)
     err, bound = (out.double() - want).abs(), off + 2.0 ** -8 * (want.abs() + off)
     assert (err <= bound).all(), f"off by {(err / bound).max()} of the bound"
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", [(1, 70, 6176), (40, 300, 8480), (100, 600, 1056), (300, 3100, 288)])
+def test_results_repeat_bit_by_bit(m, n, k, kind):
+    """Sums are joined in a fixed order, by waves, by parts of a workgroup and
+    by workgroups; two streams at once share nothing."""
+    import flashinfer_amd as fi
+
+    torch.manual_seed(0)
+    a, a_scale, _ = activations(m, k, kind)
+    b, b_scale = weights4(n, k)
+    want = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = []
+    for i in range(6):
+        with torch.cuda.stream(streams[i % 2]):
+            outs.append(fi.gemm_mxfp4_nt(a, b, b_scale, a_scale))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in outs)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale)
+    for _ in range(3):
+        out.zero_()
+        g.replay()
+        eager = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(eager, want)
 
 
 @gpu
