@@ -97,7 +97,7 @@ hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act, const voi
                          const void* a_scale, const void* b, const void* b_scale,
                          void* out, void* out_scale, float* floats, int M, int N, int K,
                          int64_t lda, int64_t ldo, hipStream_t stream);
-int64_t fi_gemm_mxfp4_floats(int a_type, int gated, int M, int N, int K);
+int64_t fi_gemm_mxfp4_floats(int a_type, int out_type, int gated, int M, int N, int K);
 hipError_t fi_per_group_quant_fp8(int dtype, int trans_scale, const void* x, void* q,
                                   float* scale, int64_t rows, int K, int64_t stride_row,
                                   float eps, hipStream_t stream);
@@ -1059,9 +1059,9 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> mxfp4_product(
                       name, ": a_scale must be contiguous uint8 [", M, ", ", K / 32, "], got ",
                       a_scale->scalar_type(), " ", a_scale->sizes());
   const int64_t N = gated ? rows / 2 : rows;
-  TORCH_CHECK_VALUE(M < (int64_t(1) << 31) && rows < (int64_t(1) << 31) &&
-                        K < (int64_t(1) << 31),
-                    name, ": a dimension passes 2^31");
+  TORCH_CHECK_VALUE(M <= (int64_t(1) << 30) && rows <= (int64_t(1) << 30) &&
+                        K <= (int64_t(1) << 30),
+                    name, ": a dimension passes 2^30");
   TORCH_CHECK_VALUE(M == 0 || (a.stride(1) == 1 &&
                                (M == 1 || (a.stride(0) >= K &&
                                            a.stride(0) * a.element_size() % 16 == 0)) &&
@@ -1124,7 +1124,7 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> mxfp4_product(
   if (quantize)
     s = out_scale ? *out_scale : empty_like_on(a, {M, N / 32}, at::kByte);
   // the sums of the parts of K, where the product is split over it
-  const int64_t floats = fi_gemm_mxfp4_floats(a_type, gated, (int)M, (int)N, (int)K);
+  const int64_t floats = fi_gemm_mxfp4_floats(a_type, out_type, gated, (int)M, (int)N, (int)K);
   at::Tensor sums;
   if (floats > 0) sums = empty_like_on(a, {floats}, at::kFloat);
   check_hip(fi_gemm_mxfp4(a_type, out_type, gated, (int)act, a.data_ptr(),

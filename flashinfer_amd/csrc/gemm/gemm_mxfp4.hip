@@ -18,21 +18,29 @@ struct Cost {
 };
 constexpr Cost kCosts16[] = {
     {k256x128, 256, 128, 4.1f, 14.3f, 26.8f, 1.07f}, {k128x128, 128, 128, 2.6f, 8.8f, 14.9f, 1.05f},
-    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.07f},  {k128x64x2, 128, 64, 2.6f, 4.9f, 0.f, 1.06f},
+    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.07f},  {k128x64, 128, 64, 2.6f, 4.1f, 0.f, 1.06f},
     {k64x64x4, 64, 64, 1.9f, 2.6f, 0.f, 1.13f},      {k64x32x4, 64, 32, 1.4f, 1.8f, 0.f, 1.15f},
     {k128x32x4, 128, 32, 1.9f, 2.9f, 0.f, 1.1f},
 };
 constexpr Cost kCosts8[] = {
     {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.22f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.11f},
-    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.26f}, {k128x64x2, 128, 64, 1.9f, 2.7f, 0.f, 1.41f},
+    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.26f}, {k128x64, 128, 64, 1.9f, 2.7f, 0.f, 1.41f},
     {k64x64x4, 64, 64, 1.7f, 1.7f, 0.f, 1.21f},     {k64x32x4, 64, 32, 0.8f, 1.5f, 0.f, 1.13f},
     {k128x32x4, 128, 32, 1.3f, 2.2f, 0.f, 1.26f},
+};
+
+// 8 bits in and out, where the small tiles widen their operands
+constexpr Cost kCosts8to8[] = {
+    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.22f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.11f},
+    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.26f}, {k128x64, 128, 64, 2.1f, 3.7f, 0.f, 1.2f},
+    {k64x64x4, 64, 64, 1.7f, 2.1f, 0.f, 1.21f},     {k64x32x4, 64, 32, 0.8f, 1.6f, 0.f, 1.13f},
+    {k128x32x4, 128, 32, 1.3f, 2.4f, 0.f, 1.26f},
 };
 
 // The kernel and tile of the least cost, and in how many parts of K the tiles
 // are computed. Parts cost a second kernel (3 us) and the way of their sums
 // through memory.
-Plan make_plan(int M, int N, int K, bool gated, bool act8) {
+Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
   if (M <= 16) return {kRows, 1, 0};
   constexpr int kCus = kNumCU, kMostParts = 16;
   const int64_t rows = gated ? 2 * (int64_t)N : N;
@@ -40,8 +48,10 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8) {
   const bool odd = K % (act8 ? 128 : 64) != 0;
   Plan best{kRows, 1, 0};
   float least = 0.f;
-  for (int i = 0; i < 7; ++i) {
-    const Cost& c = act8 ? kCosts8[i] : kCosts16[i];
+  const Cost* costs = !act8 ? kCosts16 : out8 ? kCosts8to8 : kCosts8;
+  // the first three tiles do not widen 8-bit operands
+  for (int i = act8 && out8 && M <= 128 ? 3 : 0; i < 7; ++i) {
+    const Cost& c = costs[i];
     const int64_t tiles = ceil_div64(rows, c.rows) * ceil_div64(M, c.tokens);
     for (int parts = 1; parts <= kMostParts && parts <= loads; ++parts) {
       if (parts > 1 && tiles * parts > 2 * kCus) break;
@@ -64,8 +74,10 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8) {
 }  // namespace fi
 
 // How many floats of workspace fi_gemm_mxfp4 wants for this product.
-extern "C" int64_t fi_gemm_mxfp4_floats(int a_type, int gated, int M, int N, int K) {
-  return M > 0 && N > 0 ? fi::mx4::make_plan(M, N, K, gated, a_type == fi::mx4::kFp8).floats : 0;
+extern "C" int64_t fi_gemm_mxfp4_floats(int a_type, int out_type, int gated, int M, int N, int K) {
+  using namespace fi::mx4;
+  if (M <= 0 || N <= 0) return 0;
+  return make_plan(M, N, K, gated, a_type == kFp8, out_type == kFp8).floats;
 }
 
 // a_type: 0 bf16, 1 fp16, 2 e4m3 with scale bytes; out_type the same, 2 for the
@@ -94,7 +106,7 @@ extern "C" hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act
     }
     return hipErrorInvalidValue;
   };
-  const Plan plan = make_plan(M, N, K, gated, a_type == kFp8);
+  const Plan plan = make_plan(M, N, K, gated, a_type == kFp8, out_type == kFp8);
   if (plan.parts > 1 && !floats) return hipErrorInvalidValue;
   const int a_size = a_type == kFp8 ? 1 : 2, out_size = out_type == kFp8 ? 1 : 2;
   // A tile counts its bytes in 32 bits. Rows further apart than that allows go
