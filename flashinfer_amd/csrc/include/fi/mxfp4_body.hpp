@@ -27,10 +27,10 @@
 // it costs 48 x 14336 x 4096 20.4 for 15.8 us. For more tokens, where it would
 // halve the rate, the 8-bit products stay.
 #pragma once
-#include "fi/common.hpp"
-#include "fi/mfma.hpp"
 #include <type_traits>
 
+#include "fi/common.hpp"
+#include "fi/mfma.hpp"
 #include "fi/mx.hpp"
 
 namespace fi {
@@ -493,8 +493,19 @@ hipError_t launch_rows(const Params& p, hipStream_t stream) {
 // Many tokens: a workgroup of GN x GM waves computes a tile of GN * WN * 32
 // weight rows by GM * WM * 32 tokens in 32x32 products. Steps of 128 bytes of
 // a token row (128 values in 8 bits, 64 in 16) go to shared memory with their
-// weights, several buffers in turn, by loads that bypass the registers; the scales
-// of 512 values of a row come as 16 bytes once per 512.
+// weights, several buffers in turn, by loads that bypass the registers; the
+// scales of 512 values of a row come as 16 bytes once per 512.
+//
+// 256 x 128, two on a CU: 4096 x 4096 x 14336 with 8-bit tokens takes 198 us, 2.43
+// PFLOP/s (a library product of 8-bit matrices reaches 2.61 on 8192^3); a gated
+// block of 2047 x 14336 x 4096 with bf16 tokens 380 us, 1.27 (1.41). Staging a
+// quarter of the tokens only would save a fifth of that, of the weights a
+// twelfth: what is left is the way of the operands from the L2 cache. Three
+// buffers and counted waits brought 311 -> 229 us, outputs through shared
+// memory 239 -> 197. Eight waves at 256 x 256 and waves of higher priority
+// during their products brought nothing.
+// Small tiles are bound by their tokens' way from L2 as well (47 to 59 bytes a
+// nanosecond for a CU), or, with less than 256 of them, by the latency of a step.
 //
 // Operand map of 32x32: lane l holds row (token) l & 31 and, with g = l >> 5,
 //   8-bit a, 32x32x64: fp4 k = 32g..32g+31; fp8 k = 16g..16g+15 and 32+16g..;
@@ -751,7 +762,7 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
         uint32_t ws[WN];
 #pragma unroll
         for (int i = 0; i < WN; ++i) ws[i] = ls[b_row + i * 32] >> (8 * g);
-          if constexpr (kWiden) {
+        if constexpr (kWiden) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             uint4 w[WN], x[WM][2];
@@ -900,7 +911,7 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
   else pass(std::false_type());
   // fp16: where some weight of the tile is not exact in fp16 all of it is
   // computed again with a split in two. Every wave sees the same flag.
-  if (ACT == kFp16 && *(volatile int*)&flag) {
+  if (ACT == kFp16 && __builtin_amdgcn_readfirstlane(*(volatile int*)&flag)) {
     __syncthreads();
     if (helps) bring_scales();
     else pass(std::integral_constant<bool, ACT == kFp16>());
