@@ -17,14 +17,15 @@
 //     product i takes k = 32g + 8i .. 32g + 8i + 7 from lane group g.
 //   fp16 a: the same in fp16 where every scale of the wave's chunk keeps the
 //     weights exact in fp16 (2^-23 .. 2^13); elsewhere a is split into two
-//     bf16 parts, high and low, which hold its 11 bits exactly.
+//     bf16 parts, high and low, which hold its 11 bits exactly (a tile of many
+//     tokens is then taken once more from the start).
 // The products' sums are held in 32 bits. Within one instruction the matrix
 // unit aligns 8-bit products to the largest of them, which costs about 1e-5 of
 // the result on normal data. An output in 16 bits rounds to 4e-3 or 5e-4 and
 // hides it; an MXFP8 output has scales, and one block in 50,000 would get the
 // neighbour of its own. There, up to 128 tokens, both operands become bf16 (an
 // exact step) and the error is that of 32 bits: memory bounds those sizes, and
-// it costs 48 x 14336 x 4096 20.4 for 15.8 us. For more tokens, where it would
+// it costs 48 x 14336 x 4096 19.7 for 15.8 us. For more tokens, where it would
 // halve the rate, the 8-bit products stay.
 #pragma once
 #include <type_traits>
