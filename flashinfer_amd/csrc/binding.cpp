@@ -1059,9 +1059,11 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> mxfp4_product(
                       name, ": a_scale must be contiguous uint8 [", M, ", ", K / 32, "], got ",
                       a_scale->scalar_type(), " ", a_scale->sizes());
   const int64_t N = gated ? rows / 2 : rows;
-  TORCH_CHECK_VALUE(M <= (int64_t(1) << 30) && rows <= (int64_t(1) << 30) &&
-                        K <= (int64_t(1) << 30),
-                    name, ": a dimension passes 2^30");
+  // the rows of a launch of 2^32 threads, and a row's bytes in 31 bits
+  TORCH_CHECK_VALUE(M <= (int64_t(1) << 30) && rows <= (int64_t(1) << 26) &&
+                        K <= (int64_t(1) << 29),
+                    name, ": M goes to 2^30, the rows of b to 2^26, K to 2^29, got ", M, ", ",
+                    rows, " and ", K);
   TORCH_CHECK_VALUE(M == 0 || (a.stride(1) == 1 &&
                                (M == 1 || (a.stride(0) >= K &&
                                            a.stride(0) * a.element_size() % 16 == 0)) &&

@@ -123,17 +123,23 @@ hipError_t launch(const void* x, void* residual, const void* w, void* out, void*
   const int nv = groups <= 512 ? 1 : groups <= 2048 ? 2 : groups <= 4096 ? 4 : 8;
   const int threads = ceil_div(ceil_div(groups, nv), kWaveSize) * kWaveSize;
   if (threads > 1024) return hipErrorInvalidValue;
+  // a launch has less than 2^32 threads: 2^21 rows at a time
+  constexpr int kRows = 1 << 21;
+  for (int64_t r = 0; r < rows; r += kRows) {
+    const int some = rows - r < kRows ? (int)(rows - r) : kRows;
 #define FI_GO(NV)                                                                       \
-  hipLaunchKernelGGL((mx_quant_kernel<T, NV, kNorm, kAdd, kAligned>), dim3(rows),       \
-                     dim3(threads), 0, stream, (const T*)x, (T*)residual, (const T*)w,  \
-                     (uint8_t*)out, (uint8_t*)scale, k, sx, sr, eps)
-  switch (nv) {
-    case 1: FI_GO(1); break;
-    case 2: FI_GO(2); break;
-    case 4: FI_GO(4); break;
-    default: FI_GO(8); break;
-  }
+  hipLaunchKernelGGL((mx_quant_kernel<T, NV, kNorm, kAdd, kAligned>), dim3(some),       \
+                     dim3(threads), 0, stream, (const T*)x + r * sx,                    \
+                     residual ? (T*)residual + r * sr : nullptr, (const T*)w,           \
+                     (uint8_t*)out + r * k, (uint8_t*)scale + r * (k / kMxBlock), k, sx, sr, eps)
+    switch (nv) {
+      case 1: FI_GO(1); break;
+      case 2: FI_GO(2); break;
+      case 4: FI_GO(4); break;
+      default: FI_GO(8); break;
+    }
 #undef FI_GO
+  }
   return hipGetLastError();
 }
 

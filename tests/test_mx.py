@@ -192,6 +192,18 @@ def test_product_refusals(what, change, gated):
 
 
 @needs_ext
+@pytest.mark.parametrize("m, n, k", [(1, 2 ** 26 + 2, 32), (1, 2, 2 ** 29 + 32)])
+def test_sizes_past_a_launch_are_refused(m, n, k):
+    import flashinfer_amd as fi
+
+    o = [torch.empty(m, k, dtype=torch.bfloat16), torch.empty(n, k // 2, dtype=torch.uint8),
+         torch.empty(n, k // 32, dtype=torch.uint8)]
+    for f in (fi.gemm_mxfp4_nt, fi.gemm_mxfp4_nt_gated):
+        with pytest.raises(ValueError, match="the rows of b to"):
+            f(*o)
+
+
+@needs_ext
 @pytest.mark.parametrize("what, kw", [
     ("out is bfloat16", dict(out_dtype=torch.float32)),
     ("out is bfloat16", dict(out_dtype=FP8)),
@@ -629,6 +641,52 @@ def test_rows_too_far_apart_for_32_bits():
     want = fi.gemm_mxfp4_nt(wide[:, :k].contiguous(), b, b_scale)
     got = fi.gemm_mxfp4_nt(wide[:, :k], b, b_scale)
     torch.testing.assert_close(got, want, rtol=2.0 ** -7, atol=1e-3)
+
+
+@gpu
+def test_more_rows_than_one_launch():
+    """2^26 workgroups of 64 lanes would be one thread more than a launch takes."""
+    import flashinfer_amd as fi
+
+    rows = 2 ** 26 + 3
+    row = torch.arange(1, 33, device="cuda", dtype=torch.bfloat16)
+    x = row * (torch.arange(rows, device="cuda") % 2 + 1).to(torch.bfloat16)[:, None]
+    w = torch.ones(32, device="cuda", dtype=torch.bfloat16)
+    for f in (lambda t: fi.mxfp8_quantize(t), lambda t: fi.rmsnorm_mxfp8_quant(t, w)):
+        q, s = f(x)
+        want_q, want_s = f(x[:2])
+        for i in range(2):
+            assert bool((q[i::2].view(torch.uint8) == want_q[i].view(torch.uint8)).all())
+            assert bool((s[i::2] == want_s[i]).all())
+
+
+@gpu
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("m, n", [(33000, 65600), (16, 2 ** 25)])
+def test_outputs_past_31_bits(m, n, gated):
+    """More than 2^31 outputs, or bytes of them: every row of the last columns."""
+    import flashinfer_amd as fi
+
+    torch.manual_seed(0)
+    k = 32
+    a = torch.randn(m, k, device="cuda").to(torch.bfloat16)
+    b, b_scale = weights4(64, k)
+    few = (b, b_scale)
+    rows = 2 * n if gated else n
+    b = torch.zeros(rows, k // 2, dtype=torch.uint8, device="cuda")
+    b_scale = torch.full((rows, k // 32), 127, dtype=torch.uint8, device="cuda")
+    for at, of in ((n - 32, 0), (rows - 32, 32)) if gated else ((n - 64, 0), (n - 32, 32)):
+        b[at:at + 32], b_scale[at:at + 32] = few[0][of:of + 32], few[1][of:of + 32]
+    if gated:
+        got = fi.gemm_mxfp4_nt_gated(a, b, b_scale, out_dtype=FP8)
+        want = fi.gemm_mxfp4_nt_gated(a, *few, out_dtype=FP8)
+        assert torch.equal(got[1][:, -1], want[1][:, 0])
+        assert torch.equal(got[0][:, -32:].view(torch.uint8), want[0].view(torch.uint8))
+        assert not got[0][:, :32].view(torch.uint8).any()
+    else:
+        got, want = fi.gemm_mxfp4_nt(a, b, b_scale), fi.gemm_mxfp4_nt(a, *few)
+        assert torch.equal(got[:, -64:], want)
+        assert not got[:, :64].any()
 
 
 @gpu
