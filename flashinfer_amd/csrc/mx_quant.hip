@@ -5,11 +5,11 @@
 //   y = r / sqrt(mean(r^2) + eps) * w          (y = r without a weight)
 //   2^e: the least with max|y_block| <= 448 * 2^e;   q = e4m3(y * 2^-e)
 //
-// One workgroup takes one row and keeps it in registers, eight values to a
-// lane, so every input is read once and every output written once. The four
-// lanes of a quad hold one block of 32: its maximum needs two register
-// exchanges and no shared memory. The bound is memory: 16384 x 8192 bf16 with a
-// residual takes 166 us, 5.7 TB/s, where a copy of a gigabyte reaches 5.1; an
+// One workgroup takes one row (short rows share a wave) and keeps it in
+// registers, eight values to a lane, so every input is read once and every
+// output written once. The four lanes of a quad hold one block of 32: its
+// maximum needs two register exchanges and no shared memory. The bound is memory: 16384 x 8192 bf16 with a
+// residual takes 163 us, 5.8 TB/s, where a copy of a gigabyte reaches 5.1; an
 // activation of 8191 x 14336 takes 60 us, 5.9 TB/s. Up to about 100 rows the
 // launch is the time (5 us).
 #include "fi/common.hpp"
@@ -32,21 +32,30 @@ __device__ __forceinline__ void load8(float* v, const T* p) {
   for (int j = 0; j < 8; ++j) v[j] = t.get(j);
 }
 
-// NV: groups of eight values a lane holds. kAligned: 16-byte rows.
+// NV: groups of eight values a lane holds; 0: one group, and several rows to a
+// wave, `lanes` (a power of two) for each. kAligned: 16-byte rows.
 template <typename T, int NV, bool kNorm, bool kAdd, bool kAligned>
-__global__ __launch_bounds__(1024) void mx_quant_kernel(
+__global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
     const T* __restrict__ x, T* __restrict__ residual, const T* __restrict__ w,
-    uint8_t* __restrict__ out, uint8_t* __restrict__ scale, int k, int64_t stride_x,
-    int64_t stride_r, float eps) {
+    uint8_t* __restrict__ out, uint8_t* __restrict__ scale, int rows, int k, int64_t stride_x,
+    int64_t stride_r, float eps, int lanes) {
+  constexpr bool kShort = NV == 0;
+  constexpr int kGroups = kShort ? 1 : NV;
   __shared__ float sums[16];
-  const int64_t row = blockIdx.x;
+  int64_t row = blockIdx.x;
+  int t = threadIdx.x;
+  if constexpr (kShort) {
+    row = row * (blockDim.x / lanes) + t / lanes;
+    t %= lanes;
+    if (row >= rows) return;
+  }
   const T* xr = x + row * stride_x;
   T* rr = kAdd ? residual + row * stride_r : nullptr;
-  float v[NV][8];
+  float v[kGroups][8];
   float ss = 0.f;
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (i * blockDim.x + threadIdx.x) * 8;
+  for (int i = 0; i < kGroups; ++i) {
+    const int at = (i * blockDim.x + t) * 8;
     if (at < k) {
       load8<T, kAligned>(v[i], xr + at);
       if constexpr (kAdd) {
@@ -73,17 +82,21 @@ __global__ __launch_bounds__(1024) void mx_quant_kernel(
   }
   float rrms = 1.f;
   if constexpr (kNorm) {
-    ss = wave_reduce_sum<kWaveSize>(ss);
-    const int waves = blockDim.x / kWaveSize;
-    if (threadIdx.x % kWaveSize == 0) sums[threadIdx.x / kWaveSize] = ss;
-    __syncthreads();
-    ss = 0.f;
-    for (int i = 0; i < waves; ++i) ss += sums[i];
+    if constexpr (kShort) {
+      for (int i = 1; i < lanes; i *= 2) ss += __shfl_xor(ss, i);
+    } else {
+      ss = wave_reduce_sum<kWaveSize>(ss);
+      const int waves = blockDim.x / kWaveSize;
+      if (t % kWaveSize == 0) sums[t / kWaveSize] = ss;
+      __syncthreads();
+      ss = 0.f;
+      for (int i = 0; i < waves; ++i) ss += sums[i];
+    }
     rrms = (float)(1.0 / sqrt((double)ss / k + (double)eps));
   }
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int at = (i * blockDim.x + threadIdx.x) * 8;
+  for (int i = 0; i < kGroups; ++i) {
+    const int at = (i * blockDim.x + t) * 8;
     if (at < k) {  // k is a multiple of 32: a quad is inside or outside as one
       uint32_t most = 0;
       float wv[8];
@@ -107,7 +120,7 @@ __global__ __launch_bounds__(1024) void mx_quant_kernel(
           o[4 + j] = (uint8_t)(q.y >> (8 * j));
         }
       }
-      if (threadIdx.x % 4 == 0) scale[row * (k / kMxBlock) + at / kMxBlock] = (uint8_t)byte;
+      if (t % 4 == 0) scale[row * (k / kMxBlock) + at / kMxBlock] = (uint8_t)byte;
     }
   }
 }
@@ -118,21 +131,32 @@ hipError_t launch(const void* x, void* residual, const void* w, void* out, void*
   // Two groups to a lane from 4096 values on: 512 lanes with two wait for their
   // sum with half the waves of 1024 with one (16384 x 8192: 5.7 and 5.45 TB/s,
   // 4096 x 7168: 5.6 and 5.2), and 896 lanes with two beat 448 with four
-  // (8191 x 14336: 5.55 and 5.4).
+  // (8191 x 14336: 5.55 and 5.4). Rows that leave half a wave idle share it:
+  // 262144 x 128 with a residual takes 45 us for 104, 1048576 x 64 quantized 39
+  // for 225.
   const int groups = k / 8;
-  const int nv = groups <= 512 ? 1 : groups <= 2048 ? 2 : groups <= 4096 ? 4 : 8;
-  const int threads = ceil_div(ceil_div(groups, nv), kWaveSize) * kWaveSize;
+  const int nv = groups <= kWaveSize / 2 ? 0
+                 : groups <= 512         ? 1
+                 : groups <= 2048        ? 2
+                 : groups <= 4096        ? 4
+                                         : 8;
+  int lanes = 4;
+  while (lanes < groups) lanes *= 2;
+  const int threads = nv ? ceil_div(ceil_div(groups, nv), kWaveSize) * kWaveSize : 256;
   if (threads > 1024) return hipErrorInvalidValue;
   // a launch has less than 2^32 threads: 2^21 rows at a time
   constexpr int kRows = 1 << 21;
   for (int64_t r = 0; r < rows; r += kRows) {
     const int some = rows - r < kRows ? (int)(rows - r) : kRows;
+    const int groups_of_rows = nv ? some : ceil_div(some, threads / lanes);
 #define FI_GO(NV)                                                                       \
-  hipLaunchKernelGGL((mx_quant_kernel<T, NV, kNorm, kAdd, kAligned>), dim3(some),       \
-                     dim3(threads), 0, stream, (const T*)x + r * sx,                    \
+  hipLaunchKernelGGL((mx_quant_kernel<T, NV, kNorm, kAdd, kAligned>),                   \
+                     dim3(groups_of_rows), dim3(threads), 0, stream, (const T*)x + r * sx, \
                      residual ? (T*)residual + r * sr : nullptr, (const T*)w,           \
-                     (uint8_t*)out + r * k, (uint8_t*)scale + r * (k / kMxBlock), k, sx, sr, eps)
+                     (uint8_t*)out + r * k, (uint8_t*)scale + r * (k / kMxBlock), some, \
+                     k, sx, sr, eps, lanes)
     switch (nv) {
+      case 0: FI_GO(0); break;
       case 1: FI_GO(1); break;
       case 2: FI_GO(2); break;
       case 4: FI_GO(4); break;

@@ -306,7 +306,8 @@ def to8_bits(x):
 
 @gpu
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("rows, k", [(1, 32), (3, 96), (5, 4096), (2, 8224), (2, 16416), (3, 65536)])
+@pytest.mark.parametrize("rows, k", [(1, 32), (65, 32), (33, 64), (3, 96), (19, 128), (17, 160),
+                                     (9, 256), (5, 288), (5, 4096), (2, 8224), (2, 16416), (3, 65536)])
 def test_quantize_is_exact(rows, k, dtype):
     import flashinfer_amd as fi
 
@@ -360,7 +361,8 @@ def norm_off(y, k):
 @gpu
 @pytest.mark.parametrize("add", [False, True])
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("rows, k", [(1, 32), (1, 4096), (7, 96), (33, 7168), (3, 8224), (2, 65536)])
+@pytest.mark.parametrize("rows, k", [(1, 32), (65, 32), (33, 64), (1, 4096), (7, 96), (19, 128),
+                                     (17, 160), (9, 256), (5, 288), (33, 7168), (3, 8224), (2, 65536)])
 def test_norm(rows, k, dtype, add):
     import flashinfer_amd as fi
 
@@ -399,6 +401,21 @@ def test_norm_of_zero_and_unlike_rows():
     y = norm64(x, w, 1e-6)[3:]
     check8(q[3:], s[3:], y, norm_off(y, 4096))
     assert (from8(q, s)[3:, 64:96] == 0).all()
+
+
+@gpu
+@pytest.mark.parametrize("k", [32, 64, 128, 256])
+def test_short_rows_do_not_meet(k):
+    import flashinfer_amd as fi
+
+    x = torch.randn(21, k, device="cuda", dtype=torch.bfloat16)
+    x[3, 1], x[7, k - 1] = math.nan, 1e30
+    w = torch.ones(k, device="cuda", dtype=torch.bfloat16)
+    q, s = fi.rmsnorm_mxfp8_quant(x, w)
+    assert (s[3] == 255).all()
+    rest = [i for i in range(21) if i not in (3, 7)]
+    y = norm64(x[rest], w, 1e-6)
+    check8(q[rest], s[rest], y, norm_off(y, k))
 
 
 @gpu
