@@ -247,7 +247,8 @@ struct Rows {
   static constexpr int kRing = WAVES * D * kStage;
   static constexpr int kJoin = WAVES * 16 * LD * 4;
   static constexpr int kLds = kRing + kSRows * kSRow > kJoin ? kRing + kSRows * kSRow : kJoin;
-  static constexpr int kWavesPerSimd = WAVES / 4 * (kLdsBytes / kLds < 2 ? 1 : 2);
+  static constexpr int kFit = kLdsBytes / kLds;              // workgroups that a CU has room for
+  static constexpr int kWavesPerSimd = WAVES / 4 * kFit < 4 ? WAVES / 4 * kFit : 4;
   static_assert(MR <= 16 && kLds <= kLdsBytes, "");
 };
 
@@ -401,32 +402,32 @@ void rows_kernel(Params p) {
                                                                     (int)ws[t], 0, (int)xs);
         }
       } else {
-        bool narrow = ACT == kFp16;
-        if constexpr (ACT == kFp16) {
-          bool ok = true;
+        auto weights = [&](int t, int k) {
+          return k == 0 ? w[t].x : k == 1 ? w[t].y : k == 2 ? w[t].z : w[t].w;
+        };
+        bool exact = true;
 #pragma unroll
-          for (int t = 0; t < AT; ++t) ok = ok && f16_exact(ws[t]);
-          narrow = __all(ok);
-        }
+        for (int t = 0; t < AT; ++t) exact = exact && f16_exact(ws[t]);
+        if (ACT == kFp16 && __all(exact)) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          bf16x8_t hi, lo;
-          if (ACT == kFp16 && !narrow) split_f16(x[k], hi, lo);
+          for (int k = 0; k < 4; ++k)
 #pragma unroll
-          for (int t = 0; t < AT; ++t) {
-            const uint32_t q = k == 0 ? w[t].x : k == 1 ? w[t].y : k == 2 ? w[t].z : w[t].w;
+            for (int t = 0; t < AT; ++t)
+              acc[t] = mfma_16x16x32_f16(widen_f16(weights(t, k), scale_value(ws[t])),
+                                         __builtin_bit_cast(f16x8_t, x[k]), acc[t]);
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            bf16x8_t hi = __builtin_bit_cast(bf16x8_t, x[k]), lo;
             if constexpr (ACT == kFp16) {
-              if (narrow) {
-                acc[t] = mfma_16x16x32_f16(widen_f16(q, scale_value(ws[t])),
-                                           __builtin_bit_cast(f16x8_t, x[k]), acc[t]);
-              } else {
-                const bf16x8_t wv = widen_bf16(q, scale_value(ws[t]));
-                acc[t] = mfma_16x16x32_bf16(wv, hi, acc[t]);
-                acc[t] = mfma_16x16x32_bf16(wv, lo, acc[t]);
-              }
-            } else {
-              acc[t] = mfma_16x16x32_bf16(widen_bf16(q, scale_value(ws[t])),
-                                          __builtin_bit_cast(bf16x8_t, x[k]), acc[t]);
+              __builtin_amdgcn_sched_barrier(0);  // one split's registers at a time
+              split_f16(x[k], hi, lo);
+            }
+#pragma unroll
+            for (int t = 0; t < AT; ++t) {
+              const bf16x8_t wv = widen_bf16(weights(t, k), scale_value(ws[t]));
+              acc[t] = mfma_16x16x32_bf16(wv, hi, acc[t]);
+              if constexpr (ACT == kFp16) acc[t] = mfma_16x16x32_bf16(wv, lo, acc[t]);
             }
           }
         }
@@ -1041,11 +1042,19 @@ void tile_kernel(Params p, int tiles_n, int tiles_m) {
       }
     }
   } else {
-    // odd rows: one output a lane, so that a wave still writes 128 bytes in a row
-    for (int i = tid; i < C::TM * C::kOut; i += C::kThreads) {
-      const int ml = i / C::kOut, nl = i % C::kOut, m = m0 + ml, n = n0 + nl;
-      if (m < p.M && n < p.N)
-        ((uint16_t*)p.out)[(int64_t)m * p.ldo + n] = *(const uint16_t*)(lds + ml * kRow + nl * 2);
+    // odd rows: pieces at any address, the last of a row one by one
+    for (int i = tid; i < C::TM * kPieces; i += C::kThreads) {
+      const int ml = i / kPieces, nl = i % kPieces * kEach;
+      const int m = m0 + ml, n = n0 + nl;
+      if (m >= p.M || n >= p.N) continue;
+      const uint16_t* from = (const uint16_t*)(lds + ml * kRow) + nl;
+      uint16_t* to = (uint16_t*)p.out + (int64_t)m * p.ldo + n;
+      if (n + kEach <= p.N) {
+        const uint4 v = *(const uint4*)from;
+        __builtin_memcpy(to, &v, 16);
+      } else {
+        for (int k = 0; k < p.N - n; ++k) to[k] = from[k];
+      }
     }
   }
 }
@@ -1114,14 +1123,13 @@ __global__ __launch_bounds__(256) void join_kernel(Params p, int tiles_n, int ti
     }
   } else if (m < p.M) {
     uint16_t* o = (uint16_t*)p.out + (int64_t)m * p.ldo + n;
-    const bool whole = ((uintptr_t)p.out % 8 | p.ldo % 4) == 0;
 #pragma unroll
     for (int r = 0; r < 16; r += 4) {
       union { uint16_t v[4]; uint2 q; } t;
 #pragma unroll
       for (int k = 0; k < 4; ++k) t.v[k] = to16(y[r + k], p.out_fp16);
-      if (whole && n + 2 * r + 4 <= p.N) {
-        *(uint2*)(o + 2 * r) = t.q;
+      if (n + 2 * r + 4 <= p.N) {
+        __builtin_memcpy(o + 2 * r, &t.q, 8);  // at any address
       } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -1194,7 +1202,8 @@ hipError_t launch_out(const Plan& plan, const Params& p, hipStream_t stream) {
     case kRows: {
       constexpr int kFew = ACT == kFp8 ? 8 : 4;  // tokens in a kilobyte of a chunk
       if (p.M <= kFew) return choose_rows<ACT, GATED, OUT8, 1>(p, stream);
-      return choose_rows<ACT, GATED, OUT8, ACT == kFp8 ? 2 : 4>(p, stream);
+      if (p.M <= 2 * kFew) return choose_rows<ACT, GATED, OUT8, 2>(p, stream);
+      return choose_rows<ACT, GATED, OUT8, 16 / kFew>(p, stream);
     }
     case k256x128: return launch_tile<ACT, GATED, OUT8, 2, 4, 4, 1, 1>(p, plan.parts, stream);
     case k128x128: return launch_tile<ACT, GATED, OUT8, 2, 2, 2, 2, 1>(p, plan.parts, stream);
