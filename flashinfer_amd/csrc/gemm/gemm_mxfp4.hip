@@ -37,6 +37,17 @@ constexpr Cost kCosts8to8[] = {
     {k128x32x4, 128, 32, 1.3f, 2.4f, 0.f, 1.26f},
 };
 
+// The same for rows_kernel with 17 to 32 tokens and with 33 to 64: a workgroup
+// that takes one tile of 16 weight rows, and one that takes two. Fitted to N = 4096
+// to 28672, K = 4096 to 14336. 6144 x 4096 with 32 and 64 bf16 tokens takes 7.4 and
+// 10.7 us where the best tile takes 11.3 and 11.6; 8-bit tokens 5.9 and 8.0 for 9.5
+// and 9.7. Larger products read their tokens too often (28672 x 4096 20 for 17 us).
+struct FewCost {
+  float start1, one1, start2, one2, two2;
+};
+constexpr FewCost kFew16[] = {{0.5f, 0.87f, 0.3f, 1.25f, 2.1f}, {1.6f, 1.49f, 0.8f, 1.93f, 3.3f}};
+constexpr FewCost kFew8[] = {{0.6f, 0.6f, 0.f, 1.f, 1.5f}, {1.7f, 0.89f, 0.5f, 1.3f, 2.4f}};
+
 // The kernel and tile of the least cost, and in how many parts of K the tiles
 // are computed. Parts cost a second kernel (3 us) and the way of their sums
 // through memory.
@@ -47,7 +58,15 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
   const int loads = ceil_div(K, 512);  // of scales; a part holds whole ones
   const bool odd = K % (act8 ? 128 : 64) != 0;
   Plan best{kRows, 1, 0};
-  float least = 0.f;
+  float least = -1.f;
+  if (M <= 64 && !out8) {
+    const FewCost& c = (act8 ? kFew8 : kFew16)[M > 32];
+    const float k = K / 1024.f;
+    const int64_t pairs = ceil_div64(rows, 32), each = ceil_div64(pairs, kCus);
+    least = pairs < kFewPairs && !gated
+                ? c.start1 + c.one1 * k
+                : each / 2 * (c.start2 + c.two2 * k) + each % 2 * (c.start2 + c.one2 * k);
+  }
   const Cost* costs = !act8 ? kCosts16 : out8 ? kCosts8to8 : kCosts8;
   // the first three tiles do not widen 8-bit operands
   for (int i = act8 && out8 && M <= 128 ? 3 : 0; i < 7; ++i) {
@@ -61,7 +80,7 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
                              : each * (c.start + c.one * k);
       const int64_t floats = parts > 1 ? parts * tiles * c.rows * c.tokens : 0;
       if (parts > 1) us += 3.f + floats * 8 / 3e6f;
-      if (best.shape == kRows || us < least) {
+      if (least < 0.f || us < least) {
         least = us;
         best = {c.shape, parts, floats};
       }

@@ -226,8 +226,9 @@ __device__ __forceinline__ void load_scales(uint32_t (&v)[4], const uint8_t* row
 }
 
 // ---------------------------------------------------------------------------
-// Few tokens (16 at most): the weights' bytes are what the time goes to, and
-// how many of them are on their way at once decides how fast they come. A
+// Few tokens (64 at most): the weights' bytes are what the time goes to, and
+// how many of them are on their way at once decides how fast they come. (From
+// 17 tokens on it is the tokens' way from L2 to every CU.) A
 // workgroup of WAVES waves takes RT * 16 outputs and shares K among its waves
 // in chunks of 128. Each wave has D chunks of weights (AT KB) and tokens (XI
 // KB) on their way to its own part of shared memory, by loads that bypass the
@@ -238,25 +239,26 @@ template <int ACT, bool GATED, int RT, int XI, int WAVES, int D>
 struct Rows {
   static constexpr int AT = GATED ? 2 * RT : RT;             // tiles of 16 weight rows
   static constexpr int kXRow = ACT == kFp8 ? 128 : 256;      // bytes of a token in a chunk
-  static constexpr int MR = XI * 1024 / kXRow;               // tokens held, 16 at most
+  static constexpr int MR = XI * 1024 / kXRow;               // tokens held, 64 at most
+  static constexpr int MT = (MR + 15) / 16;                  // tiles of 16 tokens
   static constexpr int kStage = (AT + XI) * 1024;
   static constexpr int kSlab = 192;                          // blocks of K with resident scales
   static constexpr int kSRow = kSlab + 16;                   // one unit more: rows in unlike banks
   static constexpr int kSRows = AT * 16 + (ACT == kFp8 ? MR : 0);
   static constexpr int LD = AT * 16 + 4;                     // of the sums to be joined
   static constexpr int kRing = WAVES * D * kStage;
-  static constexpr int kJoin = WAVES * 16 * LD * 4;
+  static constexpr int kJoin = WAVES * MT * 16 * LD * 4;
   static constexpr int kLds = kRing + kSRows * kSRow > kJoin ? kRing + kSRows * kSRow : kJoin;
   static constexpr int kFit = kLdsBytes / kLds;              // workgroups that a CU has room for
   static constexpr int kWavesPerSimd = WAVES / 4 * kFit < 4 ? WAVES / 4 * kFit : 4;
-  static_assert(MR <= 16 && kLds <= kLdsBytes, "");
+  static_assert(MR <= 64 && kLds <= kLdsBytes, "");
 };
 
 template <int ACT, bool GATED, bool OUT8, int RT, int XI, int WAVES, int D>
 __global__ __launch_bounds__(WAVES * 64, (Rows<ACT, GATED, RT, XI, WAVES, D>::kWavesPerSimd))
 void rows_kernel(Params p) {
   using C = Rows<ACT, GATED, RT, XI, WAVES, D>;
-  constexpr int AT = C::AT;
+  constexpr int AT = C::AT, MT = C::MT;
   constexpr bool kWiden = ACT == kFp8 && OUT8;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[C::kLds];
   uint8_t* const lds_s = lds + C::kRing;
@@ -306,11 +308,13 @@ void rows_kernel(Params p) {
   // where a lane reads: its weights' block, and its token's values. A column
   // of no token reads some other token; its sums are not used.
   const uint32_t read_b = spread(lr * 64 + g * 16);
-  const int xr = lr & (C::MR - 1);
+  auto token = [&](int j) { return (j * 16 + lr) & (C::MR - 1); };
 
-  floatx4 acc[AT];
+  floatx4 acc[AT][MT];
 #pragma unroll
-  for (int t = 0; t < AT; ++t) acc[t] = floatx4{0.f, 0.f, 0.f, 0.f};
+  for (int t = 0; t < AT; ++t)
+#pragma unroll
+    for (int j = 0; j < MT; ++j) acc[t][j] = floatx4{0.f, 0.f, 0.f, 0.f};
 
   for (int s0 = 0; s0 < blocks; s0 += C::kSlab) {
     const int width = blocks - s0 < C::kSlab ? blocks - s0 : C::kSlab;
@@ -359,14 +363,17 @@ void rows_kernel(Params p) {
         ws[t] = lds_s[(t * 16 + lr) * C::kSRow + c * 4 + g];
       }
       constexpr int XU = ACT == kFp8 ? 2 : 4;  // 16-byte units of a token a lane takes
-      uint4 x[XU];
-      uint32_t xs = 127;
+      uint4 x[MT][XU];
+      uint32_t xs[MT];
 #pragma unroll
-      for (int k = 0; k < XU; ++k) {
-        const int byte = kWiden ? g * 32 + k * 16 : ACT == kFp8 ? g * 16 + k * 64 : g * 64 + k * 16;
-        x[k] = *(const uint4*)(from + AT * 1024 + spread(xr * C::kXRow + byte));
+      for (int j = 0; j < MT; ++j) {
+#pragma unroll
+        for (int k = 0; k < XU; ++k) {
+          const int byte = kWiden ? g * 32 + k * 16 : ACT == kFp8 ? g * 16 + k * 64 : g * 64 + k * 16;
+          x[j][k] = *(const uint4*)(from + AT * 1024 + spread(token(j) * C::kXRow + byte));
+        }
+        if constexpr (ACT == kFp8) xs[j] = lds_s[(AT * 16 + token(j)) * C::kSRow + c * 4 + g];
       }
-      if constexpr (ACT == kFp8) xs = lds_s[(AT * 16 + xr) * C::kSRow + c * 4 + g];
       // all read: the place may be filled again
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (i + D < mine) stage(c0 + c + D * WAVES, slot);
@@ -379,32 +386,44 @@ void rows_kernel(Params p) {
           if (g >= left) w[t] = make_uint4(0, 0, 0, 0);
 #pragma unroll
         for (int k = 0; k < XU; ++k)
-          if ((ACT == kFp8 && !kWiden ? k * 2 + g / 2 : g) >= left) x[k] = make_uint4(0, 0, 0, 0);
+          if ((ACT == kFp8 && !kWiden ? k * 2 + g / 2 : g) >= left) {
+#pragma unroll
+            for (int j = 0; j < MT; ++j) x[j][k] = make_uint4(0, 0, 0, 0);
+          }
       }
+      auto weights = [&](int t, int k) {
+        return k == 0 ? w[t].x : k == 1 ? w[t].y : k == 2 ? w[t].z : w[t].w;
+      };
       if constexpr (kWiden) {
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
-          const uint4 h = x[k / 2];
-          const bf16x8_t xv = widen_fp8(k % 2 ? h.z : h.x, k % 2 ? h.w : h.y, scale_value(xs));
+          bf16x8_t xv[MT];
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            const uint4 h = x[j][k / 2];
+            xv[j] = widen_fp8(k % 2 ? h.z : h.x, k % 2 ? h.w : h.y, scale_value(xs[j]));
+          }
 #pragma unroll
           for (int t = 0; t < AT; ++t) {
-            const uint32_t q = k == 0 ? w[t].x : k == 1 ? w[t].y : k == 2 ? w[t].z : w[t].w;
-            acc[t] = mfma_16x16x32_bf16(widen_bf16(q, scale_value(ws[t])), xv, acc[t]);
+            const bf16x8_t wv = widen_bf16(weights(t, k), scale_value(ws[t]));
+#pragma unroll
+            for (int j = 0; j < MT; ++j) acc[t][j] = mfma_16x16x32_bf16(wv, xv[j], acc[t][j]);
           }
         }
       } else if constexpr (ACT == kFp8) {
-        const intx8 xv = {(int)x[0].x, (int)x[0].y, (int)x[0].z, (int)x[0].w,
-                          (int)x[1].x, (int)x[1].y, (int)x[1].z, (int)x[1].w};
 #pragma unroll
         for (int t = 0; t < AT; ++t) {
           const intx8 wv = {(int)w[t].x, (int)w[t].y, (int)w[t].z, (int)w[t].w, 0, 0, 0, 0};
-          acc[t] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wv, xv, acc[t], 4, 0, 0,
-                                                                    (int)ws[t], 0, (int)xs);
+#pragma unroll
+          for (int j = 0; j < MT; ++j) {
+            const uint4 u = x[j][0], v = x[j][1];
+            const intx8 xv = {(int)u.x, (int)u.y, (int)u.z, (int)u.w,
+                              (int)v.x, (int)v.y, (int)v.z, (int)v.w};
+            acc[t][j] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+                wv, xv, acc[t][j], 4, 0, 0, (int)ws[t], 0, (int)xs[j]);
+          }
         }
       } else {
-        auto weights = [&](int t, int k) {
-          return k == 0 ? w[t].x : k == 1 ? w[t].y : k == 2 ? w[t].z : w[t].w;
-        };
         bool exact = true;
 #pragma unroll
         for (int t = 0; t < AT; ++t) exact = exact && f16_exact(ws[t]);
@@ -412,22 +431,29 @@ void rows_kernel(Params p) {
 #pragma unroll
           for (int k = 0; k < 4; ++k)
 #pragma unroll
-            for (int t = 0; t < AT; ++t)
-              acc[t] = mfma_16x16x32_f16(widen_f16(weights(t, k), scale_value(ws[t])),
-                                         __builtin_bit_cast(f16x8_t, x[k]), acc[t]);
+            for (int t = 0; t < AT; ++t) {
+              const f16x8_t wv = widen_f16(weights(t, k), scale_value(ws[t]));
+#pragma unroll
+              for (int j = 0; j < MT; ++j)
+                acc[t][j] =
+                    mfma_16x16x32_f16(wv, __builtin_bit_cast(f16x8_t, x[j][k]), acc[t][j]);
+            }
         } else {
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
-            bf16x8_t hi = __builtin_bit_cast(bf16x8_t, x[k]), lo;
-            if constexpr (ACT == kFp16) {
-              __builtin_amdgcn_sched_barrier(0);  // one split's registers at a time
-              split_f16(x[k], hi, lo);
-            }
 #pragma unroll
-            for (int t = 0; t < AT; ++t) {
-              const bf16x8_t wv = widen_bf16(weights(t, k), scale_value(ws[t]));
-              acc[t] = mfma_16x16x32_bf16(wv, hi, acc[t]);
-              if constexpr (ACT == kFp16) acc[t] = mfma_16x16x32_bf16(wv, lo, acc[t]);
+            for (int j = 0; j < MT; ++j) {
+              bf16x8_t hi = __builtin_bit_cast(bf16x8_t, x[j][k]), lo;
+              if constexpr (ACT == kFp16) {
+                __builtin_amdgcn_sched_barrier(0);  // one split's registers at a time
+                split_f16(x[j][k], hi, lo);
+              }
+#pragma unroll
+              for (int t = 0; t < AT; ++t) {
+                const bf16x8_t wv = widen_bf16(weights(t, k), scale_value(ws[t]));
+                acc[t][j] = mfma_16x16x32_bf16(wv, hi, acc[t][j]);
+                if constexpr (ACT == kFp16) acc[t][j] = mfma_16x16x32_bf16(wv, lo, acc[t][j]);
+              }
             }
           }
         }
@@ -441,15 +467,17 @@ void rows_kernel(Params p) {
   float* const join = (float*)lds;
 #pragma unroll
   for (int t = 0; t < AT; ++t)
-    *(floatx4*)(join + (wave * 16 + lr) * C::LD + t * 16 + g * 4) = acc[t];
+#pragma unroll
+    for (int j = 0; j < MT; ++j)
+      *(floatx4*)(join + ((wave * MT + j) * 16 + lr) * C::LD + t * 16 + g * 4) = acc[t][j];
   __syncthreads();
 
   auto joined = [&](int m, int nl) {
     float s = 0.f, u = 0.f;
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) {
-      s += join[(w * 16 + m) * C::LD + nl];
-      if constexpr (GATED) u += join[(w * 16 + m) * C::LD + RT * 16 + nl];
+      s += join[(w * MT * 16 + m) * C::LD + nl];
+      if constexpr (GATED) u += join[(w * MT * 16 + m) * C::LD + RT * 16 + nl];
     }
     return GATED ? activate(p.act, s) * u : s;
   };
@@ -457,7 +485,7 @@ void rows_kernel(Params p) {
     // Eight neighbouring outputs of one token to a thread: a quad holds one
     // block. N is a multiple of 32 here.
     constexpr int G8 = RT * 2;
-    for (int i = tid; i < 16 * G8; i += WAVES * 64) {
+    for (int i = tid; i < MT * 16 * G8; i += WAVES * 64) {
       const int m = i / G8, nl = (i % G8) * 8, n = n0 + nl;
       float y[8];
       uint32_t most = 0;
@@ -476,7 +504,7 @@ void rows_kernel(Params p) {
       }
     }
   } else {
-    for (int i = tid; i < 16 * RT * 16; i += WAVES * 64) {
+    for (int i = tid; i < MT * 16 * RT * 16; i += WAVES * 64) {
       const int m = i / (RT * 16), nl = i % (RT * 16), n = n0 + nl;
       if (m < p.M && n < p.N)
         ((uint16_t*)p.out)[(int64_t)m * p.ldo + n] = to16(joined(m, nl), p.out_fp16);
@@ -1158,7 +1186,7 @@ hipError_t launch_tile(const Params& p, int parts, hipStream_t stream) {
 // Which kernel, tile and parts of K a product gets.
 
 enum Shape {
-  kRows,      // 16 tokens at most
+  kRows,      // 64 tokens at most, 16 with an MXFP8 output
   k256x128,   // weight rows x tokens, one part of K in a workgroup
   k128x128,
   k128x128x2, // two parts of K in a workgroup
@@ -1180,7 +1208,12 @@ struct Plan {
 // workgroups need many waves each; many of them hide each other's start, and
 // shared memory that is spent on chunks ahead keeps some of them out. Four
 // tiles with an MXFP8 output, (2, 8, 1) / (2, 4, 2): 4096 x 4096 7.6 / 8.2,
-// 14336 x 4096 13.2 / 12.4. Sixteen waves lose everywhere (6144 x 4096 10.2).
+// 14336 x 4096 13.2 / 12.4. Sixteen waves lose everywhere (6144 x 4096 10.2), three
+// chunks ahead as well (4096 x 14336 8.6).
+// With 17 to 64 tokens a workgroup's time is its tokens' way from L2, and two tiles
+// read them once for both as long as that leaves work for every CU: kFewPairs.
+constexpr int kFewPairs = 129;
+
 template <int ACT, bool GATED, bool OUT8, int XI>
 hipError_t choose_rows(const Params& p, hipStream_t stream) {
   if constexpr (OUT8) {
@@ -1189,9 +1222,10 @@ hipError_t choose_rows(const Params& p, hipStream_t stream) {
     return launch_rows<ACT, GATED, OUT8, 2, XI, 4, 2>(p, stream);
   } else {
     constexpr int RT = GATED ? 1 : 2;
+    constexpr bool kMany = XI * 1024 / Rows<ACT, GATED, RT, XI, 8, 1>::kXRow > 16;
     const int pairs = ceil_div(p.N, RT * 16);  // workgroups of two tiles
     if (pairs >= 512) return launch_rows<ACT, GATED, OUT8, RT, XI, 4, 1>(p, stream);
-    if (pairs < 192) return launch_rows<ACT, GATED, OUT8, 1, XI, 8, 2>(p, stream);
+    if (pairs < (kMany ? kFewPairs : 192)) return launch_rows<ACT, GATED, OUT8, 1, XI, 8, XI < 8 ? 2 : 1>(p, stream);
     return launch_rows<ACT, GATED, OUT8, RT, XI, 8, 1>(p, stream);
   }
 }
@@ -1203,7 +1237,12 @@ hipError_t launch_out(const Plan& plan, const Params& p, hipStream_t stream) {
       constexpr int kFew = ACT == kFp8 ? 8 : 4;  // tokens in a kilobyte of a chunk
       if (p.M <= kFew) return choose_rows<ACT, GATED, OUT8, 1>(p, stream);
       if (p.M <= 2 * kFew) return choose_rows<ACT, GATED, OUT8, 2>(p, stream);
-      return choose_rows<ACT, GATED, OUT8, 16 / kFew>(p, stream);
+      if (p.M <= 16) return choose_rows<ACT, GATED, OUT8, 16 / kFew>(p, stream);
+      if constexpr (!OUT8) {
+        if (p.M <= 32) return choose_rows<ACT, GATED, OUT8, 32 / kFew>(p, stream);
+        if (p.M <= 64) return choose_rows<ACT, GATED, OUT8, 64 / kFew>(p, stream);
+      }
+      return hipErrorInvalidValue;
     }
     case k256x128: return launch_tile<ACT, GATED, OUT8, 2, 4, 4, 1, 1>(p, plan.parts, stream);
     case k128x128: return launch_tile<ACT, GATED, OUT8, 2, 2, 2, 2, 1>(p, plan.parts, stream);

@@ -460,17 +460,22 @@ SHAPES = [(1, 1, 32), (1, 64, 4096), (3, 17, 160), (16, 100, 512), (17, 33, 1056
 # one for each tile, with edges on every side: 128 x 32, 64 x 32 and 64 x 64 in
 # parts of K, 64 x 64, 128 x 64, 128 x 128 in two and one parts, 256 x 128
 TILES = [(24, 25000, 64), (20, 100, 9248), (40, 300, 8480), (200, 3100, 288), (33, 20500, 160),
-         (100, 21000, 96), (520, 8450, 96), (1300, 13002, 608)]
+         (100, 21000, 96), (520, 8450, 96), (1300, 13002, 608), (100, 8200, 96), (70, 8200, 96),
+         (70, 6100, 1056)]
 
 
 # the kernel for few tokens: K in one, two and three slabs of scales, and the
 # three ways to share it
-FEW = [(1, 70, 12320), (5, 40, 6176), (16, 33, 14336), (3, 16500, 6240), (2, 7001, 96), (9, 7000, 6144)]
+FEW = [(1, 70, 12320), (5, 40, 6176), (16, 33, 14336), (3, 16500, 6240), (2, 7001, 96), (9, 7000, 6144),
+       (8, 33, 14336), (6, 7001, 96), (7, 16500, 160)]
+# the same with 17 to 32 tokens and 33 to 64
+MORE = [(20, 2001, 6240), (32, 5000, 6176), (17, 16600, 160), (32, 4100, 96), (40, 4090, 6176),
+        (64, 5003, 416), (33, 17000, 96), (64, 4113, 6176)]
 
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-@pytest.mark.parametrize("m, n, k", SHAPES + TILES + FEW)
+@pytest.mark.parametrize("m, n, k", SHAPES + TILES + FEW + MORE)
 def test_gemm(m, n, k, kind):
     import flashinfer_amd as fi
 
@@ -518,14 +523,15 @@ def test_gated(m, n, k, kind, act):
 
 
 @gpu
+@pytest.mark.parametrize("m", [12, 20, 50, 90])
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-def test_every_scale_and_special_values(kind):
+def test_every_scale_and_special_values(kind, m):
     """Scales from the least to the largest that keep the result finite, NaN
     scales, and NaN and infinite activations."""
     import flashinfer_amd as fi
 
     torch.manual_seed(0)
-    m, n, k = 20, 200, 256
+    n, k = 200, 256
     a, a_scale, a64 = activations(m, k, kind)
     b, _ = weights4(n, k)
     b_scale = torch.arange(n, device="cuda").to(torch.uint8).unsqueeze(1).repeat(1, k // BLOCK)
@@ -572,7 +578,9 @@ def test_every_scale_and_special_values(kind):
 @pytest.mark.parametrize("m, n, k", [(24, 12512, 64), (20, 64, 9248), (40, 160, 8480), (200, 1568, 288),
                                      (33, 10272, 160), (100, 10528, 96), (520, 4256, 96),
                                      (1300, 6528, 608), (1, 64, 12320), (16, 32, 6176), (5, 12320, 160),
-                                     (3, 16512, 96)])
+                                     (3, 16512, 96), (8, 32, 6176), (20, 2592, 6176), (24, 4128, 416),
+                                     (32, 8224, 96), (64, 2080, 6240), (50, 8224, 96), (48, 608, 96),
+                                     (100, 4192, 96), (70, 4224, 96)])
 def test_gated_tiles(m, n, k, kind):
     import flashinfer_amd as fi
 
@@ -594,6 +602,7 @@ def test_gated_tiles(m, n, k, kind):
 
 @gpu
 @pytest.mark.parametrize("m, n, k", [(3, 40, 160), (24, 12500, 64), (40, 300, 8480), (200, 3100, 288),
+                                     (32, 5000, 416), (60, 5000, 416), (70, 8200, 96), (100, 8200, 96),
                                      (100, 10500, 96), (520, 8450, 96), (1300, 13002, 96)])
 def test_fp16_with_weights_outside_its_range(m, n, k):
     """Blocks whose weights fp16 does not hold, some of a tile and some tiles:
@@ -616,7 +625,8 @@ def test_fp16_with_weights_outside_its_range(m, n, k):
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-@pytest.mark.parametrize("m, n, k", [(1, 70, 6176), (40, 300, 8480), (100, 600, 1056), (300, 3100, 288)])
+@pytest.mark.parametrize("m, n, k", [(1, 70, 6176), (40, 300, 8480), (100, 600, 1056), (300, 3100, 288),
+                                     (30, 5000, 6176), (60, 5000, 416)])
 def test_results_repeat_bit_by_bit(m, n, k, kind):
     """Sums are joined in a fixed order, by waves, by parts of a workgroup and
     by workgroups; two streams at once share nothing."""
@@ -708,7 +718,7 @@ def test_outputs_past_31_bits(m, n, gated):
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-@pytest.mark.parametrize("m", [1, 16, 40, 300])
+@pytest.mark.parametrize("m", [1, 16, 24, 40, 300])
 def test_rows_apart_and_outputs_given(m, kind):
     """Strided rows of a, an output inside a wider tensor, and nothing written
     beside it; NaN lies where nothing may be read."""
