@@ -10,31 +10,31 @@ namespace mx4 {
 // with 256, 512 and 1024 tiles (each time within 17 %; 25 % for 128 x 32). Large
 // tiles move fewer bytes for a product, small ones leave fewer CUs without work.
 // `apart`: how much longer it takes where rows of a do not start at multiples of
-// 128 bytes, so that every piece of one lies in two lines (K = 7520 to 7680).
+// 128 bytes, so that every piece of one lies in two lines (K = 2080 to 7680).
 struct Cost {
   int shape, rows, tokens;
   float start, one, two;  // two: 0 where a CU has room for one
   float apart;
 };
 constexpr Cost kCosts16[] = {
-    {k256x128, 256, 128, 4.1f, 14.3f, 26.8f, 1.07f}, {k128x128, 128, 128, 2.6f, 8.8f, 14.9f, 1.05f},
-    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.07f},  {k128x64, 128, 64, 2.6f, 4.1f, 0.f, 1.06f},
-    {k64x64x4, 64, 64, 1.9f, 2.6f, 0.f, 1.13f},      {k64x32x4, 64, 32, 1.4f, 1.8f, 0.f, 1.15f},
-    {k128x32x4, 128, 32, 1.9f, 2.9f, 0.f, 1.1f},
+    {k256x128, 256, 128, 4.1f, 14.3f, 26.8f, 1.08f}, {k128x128, 128, 128, 2.6f, 8.8f, 14.9f, 1.06f},
+    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.08f},  {k128x64, 128, 64, 2.6f, 4.3f, 0.f, 1.1f},
+    {k64x64x4, 64, 64, 1.9f, 2.6f, 0.f, 1.15f},      {k64x32x4, 64, 32, 1.4f, 1.8f, 0.f, 1.17f},
+    {k128x32x4, 128, 32, 1.9f, 3.f, 0.f, 1.25f},
 };
 constexpr Cost kCosts8[] = {
-    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.22f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.11f},
-    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.26f}, {k128x64, 128, 64, 1.9f, 2.7f, 0.f, 1.41f},
-    {k64x64x4, 64, 64, 1.7f, 1.7f, 0.f, 1.21f},     {k64x32x4, 64, 32, 0.8f, 1.5f, 0.f, 1.13f},
-    {k128x32x4, 128, 32, 1.3f, 2.2f, 0.f, 1.26f},
+    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.26f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.16f},
+    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.27f}, {k128x64, 128, 64, 1.9f, 2.7f, 0.f, 1.38f},
+    {k64x64x4, 64, 64, 1.7f, 1.7f, 0.f, 1.28f},     {k64x32x4, 64, 32, 0.8f, 1.5f, 0.f, 1.22f},
+    {k128x32x4, 128, 32, 1.3f, 2.2f, 0.f, 1.33f},
 };
 
 // 8 bits in and out, where the small tiles widen their operands
 constexpr Cost kCosts8to8[] = {
-    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.22f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.11f},
-    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.26f}, {k128x64, 128, 64, 2.1f, 3.7f, 0.f, 1.2f},
-    {k64x64x4, 64, 64, 1.7f, 2.1f, 0.f, 1.21f},     {k64x32x4, 64, 32, 0.8f, 1.6f, 0.f, 1.13f},
-    {k128x32x4, 128, 32, 1.3f, 2.4f, 0.f, 1.26f},
+    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.26f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.16f},
+    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.27f}, {k128x64, 128, 64, 2.1f, 3.7f, 0.f, 1.25f},
+    {k64x64x4, 64, 64, 1.7f, 2.1f, 0.f, 1.28f},     {k64x32x4, 64, 32, 0.8f, 1.6f, 0.f, 1.22f},
+    {k128x32x4, 128, 32, 1.3f, 2.4f, 0.f, 1.33f},
 };
 
 // The same for rows_kernel with 17 to 32 tokens and with 33 to 64: a workgroup

@@ -457,11 +457,18 @@ SHAPES = [(1, 1, 32), (1, 64, 4096), (3, 17, 160), (16, 100, 512), (17, 33, 1056
           (64, 48, 2080), (65, 130, 4096), (130, 301, 544), (257, 513, 1024), (1024, 260, 288)]
 
 
-# one for each tile, with edges on every side: 128 x 32, 64 x 32 and 64 x 64 in
-# parts of K, 64 x 64, 128 x 64, 128 x 128 in two and one parts, 256 x 128
+# tiles with edges on every side, whole and in parts of K
 TILES = [(24, 25000, 64), (20, 100, 9248), (40, 300, 8480), (200, 3100, 288), (33, 20500, 160),
          (100, 21000, 96), (520, 8450, 96), (1300, 13002, 608), (100, 8200, 96), (70, 8200, 96),
          (70, 6100, 1056)]
+# and every tile again, whole and in parts of K, with 70 tokens or more
+EVERY = [(70, 96, 96), (70, 96, 4128), (100, 4256, 96), (100, 8480, 96), (70, 16512, 96),
+         (390, 16512, 96), (100, 1056, 6176), (70, 2080, 9248), (70, 8480, 96), (513, 608, 9248),
+         (100, 4256, 1056), (70, 16512, 544), (100, 8480, 9248)]
+EVERY_GATED = [(70, 96, 96), (100, 2080, 96), (70, 96, 4128), (100, 4256, 96), (200, 4256, 96),
+               (130, 16512, 96), (260, 320, 6176), (70, 1056, 9248), (100, 8480, 1056),
+               (100, 2080, 9248), (70, 4256, 96), (100, 2080, 14336), (513, 1056, 9248),
+               (513, 1056, 14336), (70, 8480, 14336)]
 
 
 # the kernel for few tokens: K in one, two and three slabs of scales, and the
@@ -475,7 +482,7 @@ MORE = [(20, 2001, 6240), (32, 5000, 6176), (17, 16600, 160), (32, 4100, 96), (4
 
 @gpu
 @pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
-@pytest.mark.parametrize("m, n, k", SHAPES + TILES + FEW + MORE)
+@pytest.mark.parametrize("m, n, k", SHAPES + TILES + EVERY + FEW + MORE)
 def test_gemm(m, n, k, kind):
     import flashinfer_amd as fi
 
@@ -580,7 +587,7 @@ def test_every_scale_and_special_values(kind, m):
                                      (1300, 6528, 608), (1, 64, 12320), (16, 32, 6176), (5, 12320, 160),
                                      (3, 16512, 96), (8, 32, 6176), (20, 2592, 6176), (24, 4128, 416),
                                      (32, 8224, 96), (64, 2080, 6240), (50, 8224, 96), (48, 608, 96),
-                                     (100, 4192, 96), (70, 4224, 96)])
+                                     (100, 4192, 96), (70, 4224, 96)] + EVERY_GATED)
 def test_gated_tiles(m, n, k, kind):
     import flashinfer_amd as fi
 
