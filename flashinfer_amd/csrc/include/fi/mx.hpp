@@ -50,4 +50,14 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
   return v > o ? v : o;
 }
 
+// Maximum over a half of the wave (lanes 0 .. 31 or 32 .. 63).
+__device__ __forceinline__ uint32_t max32(uint32_t v) {
+#pragma unroll
+  for (int i = 1; i < 32; i *= 2) {
+    const uint32_t o = (uint32_t)__shfl_xor((int)v, i);
+    v = v > o ? v : o;
+  }
+  return v;
+}
+
 }  // namespace fi

@@ -482,26 +482,17 @@ void rows_kernel(Params p) {
     return GATED ? activate(p.act, s) * u : s;
   };
   if constexpr (OUT8) {
-    // Eight neighbouring outputs of one token to a thread: a quad holds one
-    // block. N is a multiple of 32 here.
-    constexpr int G8 = RT * 2;
-    for (int i = tid; i < MT * 16 * G8; i += WAVES * 64) {
-      const int m = i / G8, nl = (i % G8) * 8, n = n0 + nl;
-      float y[8];
-      uint32_t most = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        y[j] = joined(m, nl + j);
-        most = abs_bits(y[j]) > most ? abs_bits(y[j]) : most;
-      }
-      most = quad_max(most);
-      const uint32_t byte = mxfp8_scale_byte(most);
-      if (m < p.M && n < p.N) {
-        *reinterpret_cast<uint2*>((uint8_t*)p.out + (int64_t)m * p.ldo + n) =
-            mxfp8_pack8(y, mx_inverse_scale(byte), byte == 255u);
-        if (nl % 32 == 0)
-          p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
-      }
+    // an output to a lane: 32 of them hold one block. N is a multiple of 32 here.
+    static_assert(RT == 2, "");
+    for (int i = tid; i < MT * 512; i += WAVES * 64) {
+      const int m = i / 32, nl = i % 32, n = n0 + nl;
+      if (m >= p.M) continue;
+      const float y = joined(m, nl);
+      const uint32_t byte = mxfp8_scale_byte(max32(abs_bits(y)));
+      const float q = y * mx_inverse_scale(byte);
+      const uint32_t e4m3 = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(q, q, 0, false);
+      ((uint8_t*)p.out)[(int64_t)m * p.ldo + n] = byte == 255u ? 0x7f : (uint8_t)e4m3;
+      if (nl == 0) p.out_scale[(int64_t)m * (p.N / kMxBlock) + n / kMxBlock] = (uint8_t)byte;
     }
   } else {
     for (int i = tid; i < MT * 16 * RT * 16; i += WAVES * 64) {
@@ -1207,8 +1198,9 @@ struct Plan {
 // 6.2, 12288 x 8192 14.7 / 10.9 / 11.4, 32000 x 4096 14.5 / 13.2 / 12.4. Few
 // workgroups need many waves each; many of them hide each other's start, and
 // shared memory that is spent on chunks ahead keeps some of them out. Four
-// tiles with an MXFP8 output, (2, 8, 1) / (2, 4, 2): 4096 x 4096 7.6 / 8.2,
-// 14336 x 4096 13.2 / 12.4. Sixteen waves lose everywhere (6144 x 4096 10.2), three
+// tiles with an MXFP8 output, (2, 8, 1) / (2, 4, 2): 14336 x 4096 12.3 / 12.6, 28672
+// x 8192 54.3 / 55.8; fp16 4096 x 4096 (2, 8, 2) / (2, 8, 1) 7.5 / 7.6, 16 tokens of
+// 2560 x 8192 12.5 / 14.0. Sixteen waves lose everywhere (6144 x 4096 10.2), three
 // chunks ahead as well (4096 x 14336 8.6).
 // With 17 to 64 tokens a workgroup's time is its tokens' way from L2, and two tiles
 // read them once for both as long as that leaves work for every CU: kFewPairs.
@@ -1218,7 +1210,9 @@ template <int ACT, bool GATED, bool OUT8, int XI>
 hipError_t choose_rows(const Params& p, hipStream_t stream) {
   if constexpr (OUT8) {
     // a block of the output is 32 wide: four tiles
-    if (p.N < 384 * 32) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 1>(p, stream);
+    if constexpr (ACT != kFp16) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 1>(p, stream);
+    // its two ways of widening want more registers than four waves a SIMD have
+    if (p.N <= 256 * 32) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 2>(p, stream);
     return launch_rows<ACT, GATED, OUT8, 2, XI, 4, 2>(p, stream);
   } else {
     constexpr int RT = GATED ? 1 : 2;
