@@ -37,19 +37,31 @@ constexpr Cost kCosts8to8[] = {
     {k128x32x4, 128, 32, 1.3f, 2.4f, 0.f, 1.33f},
 };
 
-// The same for rows_kernel with 17 to 32 tokens and with 33 to 64: a workgroup
-// that takes one tile of 16 weight rows, and one that takes two. Fitted to N = 4096
-// to 28672, K = 4096 to 14336. 6144 x 4096 with 32 and 64 bf16 tokens takes 7.4 and
-// 10.7 us where the best tile takes 11.3 and 11.6; 8-bit tokens 5.9 and 8.0 for 9.5
-// and 9.7. Larger products read their tokens too often (28672 x 4096 20 for 17 us).
+// The same for rows_kernel with 17 to 32 tokens and with 33 to 64, for workgroups
+// of one, two and four tiles of 16 weight rows: its time grows with the number of
+// workgroups as well, `all` of them for 1024 of K, for all read the tokens from L2.
+// Fitted to N = 512 to 28672, K = 4096 to 14336 (within 10 %). 6144 x 4096 with 32
+// and 64 bf16 tokens takes 7.2 and 10.4 us where the best tile takes 11.3 and 11.6;
+// 8-bit tokens 5.9 and 8.0 for 9.5 and 9.7. Larger products read their tokens too
+// often (28672 x 4096 20 for 17 us).
 struct FewCost {
-  float start1, one1, start2, one2, two2;
+  float start, one, all;
 };
-constexpr FewCost kFew16[] = {{0.5f, 0.87f, 0.3f, 1.25f, 2.1f}, {1.6f, 1.49f, 0.8f, 1.93f, 3.3f}};
-constexpr FewCost kFew8[] = {{0.6f, 0.6f, 0.f, 1.f, 1.5f}, {1.7f, 0.89f, 0.5f, 1.3f, 2.4f}};
+struct FewCosts {
+  FewCost by1, by2;
+  float start2, two;  // where a CU takes two of by2
+  FewCost by4;        // an MXFP8 output
+  float apart;
+};
+constexpr FewCosts kFew16[] = {
+    {{0.6f, 0.48f, 0.0016f}, {1.7f, 0.4f, 0.0026f}, 3.f, 1.5f, {1.2f, 1.14f, 0.0042f}, 1.2f},
+    {{1.7f, 0.72f, 0.003f}, {2.2f, 0.93f, 0.0032f}, 4.4f, 2.6f, {}, 1.2f}};
+constexpr FewCosts kFew8[] = {
+    {{0.7f, 0.49f, 0.0004f}, {0.f, 0.64f, 0.0016f}, 4.f, 0.7f, {1.2f, 1.f, 0.0029f}, 1.35f},
+    {{1.9f, 0.21f, 0.0026f}, {2.6f, 0.33f, 0.0027f}, 6.f, 1.f, {}, 1.35f}};
 
 // The kernel and tile of the least cost, and in how many parts of K the tiles
-// are computed. Parts cost a second kernel (3 us) and the way of their sums
+// are computed. Parts cost a second kernel (3.5 us) and the way of their sums
 // through memory.
 Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
   if (M <= 16) return {kRows, 1, 0};
@@ -59,13 +71,19 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
   const bool odd = K % (act8 ? 128 : 64) != 0;
   Plan best{kRows, 1, 0};
   float least = -1.f;
-  if (M <= 64 && !out8) {
-    const FewCost& c = (act8 ? kFew8 : kFew16)[M > 32];
-    const float k = K / 1024.f;
-    const int64_t pairs = ceil_div64(rows, 32), each = ceil_div64(pairs, kCus);
-    least = pairs < kFewPairs && !gated
-                ? c.start1 + c.one1 * k
-                : each / 2 * (c.start2 + c.two2 * k) + each % 2 * (c.start2 + c.one2 * k);
+  if (M <= (out8 ? 32 : 64)) {
+    const FewCosts& f = (act8 ? kFew8 : kFew16)[M > 32];
+    const int64_t pairs = ceil_div64(rows, 32), quads = ceil_div64(rows, 64);
+    const float k = K / 1024.f * (odd ? f.apart : 1.f);
+    auto cost = [&](const FewCost& c, int64_t all) { return c.start + (c.one + c.all * all) * k; };
+    if (out8)
+      least = ceil_div64(quads, kCus) * cost(f.by4, quads < kCus ? quads : kCus);
+    else if (pairs < kFewPairs && !gated)
+      least = cost(f.by1, 2 * pairs);
+    else if (pairs <= kCus)
+      least = cost(f.by2, pairs);
+    else
+      least = ceil_div64(pairs, 2 * kCus) * (f.start2 + f.two * k);
   }
   const Cost* costs = !act8 ? kCosts16 : out8 ? kCosts8to8 : kCosts8;
   // the first three tiles do not widen 8-bit operands
@@ -79,7 +97,7 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
       float us = c.two > 0.f ? each / 2 * (c.start + c.two * k) + each % 2 * (c.start + c.one * k)
                              : each * (c.start + c.one * k);
       const int64_t floats = parts > 1 ? parts * tiles * c.rows * c.tokens : 0;
-      if (parts > 1) us += 3.f + floats * 8 / 3e6f;
+      if (parts > 1) us += 3.5f + floats * 8 / 3e6f;
       if (least < 0.f || us < least) {
         least = us;
         best = {c.shape, parts, floats};

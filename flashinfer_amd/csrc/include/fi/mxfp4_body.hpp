@@ -1177,7 +1177,7 @@ hipError_t launch_tile(const Params& p, int parts, hipStream_t stream) {
 // Which kernel, tile and parts of K a product gets.
 
 enum Shape {
-  kRows,      // 64 tokens at most, 16 with an MXFP8 output
+  kRows,      // 64 tokens at most, 32 with an MXFP8 output
   k256x128,   // weight rows x tokens, one part of K in a workgroup
   k128x128,
   k128x128x2, // two parts of K in a workgroup
@@ -1210,10 +1210,13 @@ template <int ACT, bool GATED, bool OUT8, int XI>
 hipError_t choose_rows(const Params& p, hipStream_t stream) {
   if constexpr (OUT8) {
     // a block of the output is 32 wide: four tiles
-    if constexpr (ACT != kFp16) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 1>(p, stream);
-    // its two ways of widening want more registers than four waves a SIMD have
-    if (p.N <= 256 * 32) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 2>(p, stream);
-    return launch_rows<ACT, GATED, OUT8, 2, XI, 4, 2>(p, stream);
+    if constexpr (ACT != kFp16 || XI == 8) {
+      return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 1>(p, stream);
+    } else {
+      // its two ways of widening want more registers than four waves a SIMD have
+      if (p.N <= 256 * 32) return launch_rows<ACT, GATED, OUT8, 2, XI, 8, 2>(p, stream);
+      return launch_rows<ACT, GATED, OUT8, 2, XI, 4, 2>(p, stream);
+    }
   } else {
     constexpr int RT = GATED ? 1 : 2;
     constexpr bool kMany = XI * 1024 / Rows<ACT, GATED, RT, XI, 8, 1>::kXRow > 16;
@@ -1232,8 +1235,8 @@ hipError_t launch_out(const Plan& plan, const Params& p, hipStream_t stream) {
       if (p.M <= kFew) return choose_rows<ACT, GATED, OUT8, 1>(p, stream);
       if (p.M <= 2 * kFew) return choose_rows<ACT, GATED, OUT8, 2>(p, stream);
       if (p.M <= 16) return choose_rows<ACT, GATED, OUT8, 16 / kFew>(p, stream);
+      if (p.M <= 32) return choose_rows<ACT, GATED, OUT8, 32 / kFew>(p, stream);
       if constexpr (!OUT8) {
-        if (p.M <= 32) return choose_rows<ACT, GATED, OUT8, 32 / kFew>(p, stream);
         if (p.M <= 64) return choose_rows<ACT, GATED, OUT8, 64 / kFew>(p, stream);
       }
       return hipErrorInvalidValue;

@@ -586,7 +586,7 @@ def test_every_scale_and_special_values(kind, m):
                                      (33, 10272, 160), (100, 10528, 96), (520, 4256, 96),
                                      (1300, 6528, 608), (1, 64, 12320), (16, 32, 6176), (5, 12320, 160),
                                      (3, 16512, 96), (8, 32, 6176), (20, 2592, 6176), (24, 4128, 416),
-                                     (32, 8224, 96), (64, 2080, 6240), (50, 8224, 96), (48, 608, 96),
+                                     (32, 8224, 96), (64, 2080, 6240), (50, 8224, 96), (48, 608, 96), (24, 1056, 6176),
                                      (100, 4192, 96), (70, 4224, 96)] + EVERY_GATED)
 def test_gated_tiles(m, n, k, kind):
     import flashinfer_amd as fi
