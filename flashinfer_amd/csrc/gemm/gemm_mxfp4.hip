@@ -7,8 +7,9 @@ namespace mx4 {
 
 // What a tile costs: us to start and to finish, and us for 1024 of K where a CU
 // holds one workgroup and where it holds two. Fitted to K = 1024, 2048 and 7680
-// with 256, 512 and 1024 tiles (each time within 17 %; 25 % for 128 x 32). Large
-// tiles move fewer bytes for a product, small ones leave fewer CUs without work.
+// with 256, 512 and 1024 tiles (each time within 17 %; 25 % for 128 x 32); the
+// tile chosen is within 2 % of the best one over random products. Large tiles
+// move fewer bytes for a product, small ones leave fewer CUs without work.
 // `apart`: how much longer it takes where rows of a do not start at multiples of
 // 128 bytes, so that every piece of one lies in two lines (K = 2080 to 7680).
 struct Cost {
@@ -18,8 +19,8 @@ struct Cost {
 };
 constexpr Cost kCosts16[] = {
     {k256x128, 256, 128, 4.1f, 14.3f, 26.8f, 1.08f}, {k128x128, 128, 128, 2.6f, 8.8f, 14.9f, 1.06f},
-    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.08f},  {k128x64, 128, 64, 2.6f, 4.3f, 0.f, 1.1f},
-    {k64x64x4, 64, 64, 1.9f, 2.6f, 0.f, 1.15f},      {k64x32x4, 64, 32, 1.4f, 1.8f, 0.f, 1.17f},
+    {k128x128x2, 128, 128, 3.1f, 7.5f, 0.f, 1.08f},  {k128x64, 128, 64, 2.6f, 4.1f, 0.f, 1.13f},
+    {k64x64x4, 64, 64, 1.9f, 2.75f, 0.f, 1.15f},     {k64x32x4, 64, 32, 1.4f, 1.8f, 0.f, 1.17f},
     {k128x32x4, 128, 32, 1.9f, 3.f, 0.f, 1.25f},
 };
 constexpr Cost kCosts8[] = {
@@ -54,14 +55,14 @@ struct FewCosts {
   float apart;
 };
 constexpr FewCosts kFew16[] = {
-    {{0.6f, 0.48f, 0.0016f}, {1.7f, 0.4f, 0.0026f}, 3.f, 1.5f, {1.2f, 1.14f, 0.0042f}, 1.2f},
-    {{1.7f, 0.72f, 0.003f}, {2.2f, 0.93f, 0.0032f}, 4.4f, 2.6f, {}, 1.2f}};
+    {{0.6f, 0.48f, 0.0016f}, {1.7f, 0.4f, 0.0026f}, 2.f, 1.9f, {0.7f, 1.14f, 0.0042f}, 1.2f},
+    {{1.7f, 0.72f, 0.003f}, {1.2f, 0.93f, 0.0032f}, 4.4f, 2.6f, {}, 1.2f}};
 constexpr FewCosts kFew8[] = {
-    {{0.7f, 0.49f, 0.0004f}, {0.f, 0.64f, 0.0016f}, 4.f, 0.7f, {1.2f, 1.f, 0.0029f}, 1.35f},
-    {{1.9f, 0.21f, 0.0026f}, {2.6f, 0.33f, 0.0027f}, 6.f, 1.f, {}, 1.35f}};
+    {{0.7f, 0.49f, 0.0004f}, {0.f, 0.58f, 0.0016f}, 0.8f, 1.25f, {0.7f, 1.f, 0.0029f}, 1.35f},
+    {{1.9f, 0.5f, 0.0016f}, {2.2f, 0.6f, 0.0018f}, 6.f, 1.f, {}, 1.35f}};
 
 // The kernel and tile of the least cost, and in how many parts of K the tiles
-// are computed. Parts cost a second kernel (3.5 us) and the way of their sums
+// are computed. Parts cost a second kernel (3 us) and the way of their sums
 // through memory.
 Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
   if (M <= 16) return {kRows, 1, 0};
@@ -83,7 +84,9 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
     else if (pairs <= kCus)
       least = cost(f.by2, pairs);
     else
-      least = ceil_div64(pairs, 2 * kCus) * (f.start2 + f.two * k);
+      // a CU has room for more than two with 32 tokens, which evens out the end
+      least = (M > 32 ? ceil_div64(pairs, 2 * kCus) : pairs > 2 * kCus ? pairs / (2.f * kCus) : 1.f) *
+              (f.start2 + f.two * k);
   }
   const Cost* costs = !act8 ? kCosts16 : out8 ? kCosts8to8 : kCosts8;
   // the first three tiles do not widen 8-bit operands
@@ -97,7 +100,7 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
       float us = c.two > 0.f ? each / 2 * (c.start + c.two * k) + each % 2 * (c.start + c.one * k)
                              : each * (c.start + c.one * k);
       const int64_t floats = parts > 1 ? parts * tiles * c.rows * c.tokens : 0;
-      if (parts > 1) us += 3.5f + floats * 8 / 3e6f;
+      if (parts > 1) us += 3.f + floats * 8 / 3e6f;
       if (least < 0.f || us < least) {
         least = us;
         best = {c.shape, parts, floats};
