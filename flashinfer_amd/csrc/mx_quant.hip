@@ -8,9 +8,10 @@
 // One workgroup takes one row (short rows share a wave) and keeps it in
 // registers, eight values to a lane, so every input is read once and every
 // output written once. The four lanes of a quad hold one block of 32: its
-// maximum needs two register exchanges and no shared memory. The bound is memory: 16384 x 8192 bf16 with a
-// residual takes 163 us, 5.8 TB/s, where a copy of a gigabyte reaches 5.1; an
-// activation of 8191 x 14336 takes 60 us, 5.9 TB/s. Up to about 100 rows the
+// maximum needs two register exchanges and no shared memory. The sum of squares
+// is held in 64 bits, which costs nothing: the bound is memory. 16384 x 8192 bf16
+// with a residual takes 163 us, 5.8 TB/s, where a copy of a gigabyte reaches 5.1;
+// an activation of 8191 x 14336 takes 60 us, 5.9 TB/s. Up to about 100 rows the
 // launch is the time (5 us).
 #include "fi/common.hpp"
 #include "fi/mx.hpp"
@@ -41,7 +42,7 @@ __global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
     int64_t stride_r, float eps, int lanes) {
   constexpr bool kShort = NV == 0;
   constexpr int kGroups = kShort ? 1 : NV;
-  __shared__ float sums[16];
+  __shared__ double sums[16];
   int64_t row = blockIdx.x;
   int t = threadIdx.x;
   if constexpr (kShort) {
@@ -52,7 +53,7 @@ __global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
   const T* xr = x + row * stride_x;
   T* rr = kAdd ? residual + row * stride_r : nullptr;
   float v[kGroups][8];
-  float ss = 0.f;
+  double ss = 0.;
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int at = (i * blockDim.x + t) * 8;
@@ -76,40 +77,53 @@ __global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
       }
       if constexpr (kNorm) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) ss += v[i][j] * v[i][j];
+        for (int j = 0; j < 8; ++j) ss = __builtin_fma((double)v[i][j], (double)v[i][j], ss);
       }
     }
   }
-  float rrms = 1.f;
+  double rrms = 1.;
   if constexpr (kNorm) {
     if constexpr (kShort) {
       for (int i = 1; i < lanes; i *= 2) ss += __shfl_xor(ss, i);
     } else {
-      ss = wave_reduce_sum<kWaveSize>(ss);
+#pragma unroll
+      for (int i = 1; i < kWaveSize; i *= 2) ss += __shfl_xor(ss, i);
       const int waves = blockDim.x / kWaveSize;
       if (t % kWaveSize == 0) sums[t / kWaveSize] = ss;
       __syncthreads();
-      ss = 0.f;
+      ss = 0.;
       for (int i = 0; i < waves; ++i) ss += sums[i];
     }
-    rrms = (float)(1.0 / sqrt((double)ss / k + (double)eps));
+    rrms = 1. / sqrt(ss / k + (double)eps);
   }
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
     const int at = (i * blockDim.x + t) * 8;
     if (at < k) {  // k is a multiple of 32: a quad is inside or outside as one
       uint32_t most = 0;
-      float wv[8];
+      float wv[8], y[8];
       if constexpr (kNorm) load8<T, kAligned>(wv, w + at);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        if constexpr (kNorm) v[i][j] = v[i][j] * rrms * wv[j];
-        const uint32_t b = abs_bits(v[i][j]);
+        y[j] = kNorm ? v[i][j] * (float)rrms * wv[j] : v[i][j];
+        const uint32_t b = abs_bits(y[j]);
         most = b > most ? b : most;
       }
       most = quad_max(most);
+      if constexpr (kNorm) {
+        // Next to the border of two scales 32 bits could take the wrong one: there
+        // (one block in a million) 64 bits decide, for the quad as one.
+        if ((most & 0x7fffffu) - 0x5ffff0u <= 0x20u && most < 0x7f800000u) {
+          const double border = (double)__uint_as_float((most & 0x7f800000u) | 0x600000u);
+          uint32_t over = 0;
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            over |= __builtin_fabs((double)v[i][j] * rrms * (double)wv[j]) > border;
+          most = (most & 0x7f800000u) | (0x600000u + quad_max(over));
+        }
+      }
       const uint32_t byte = mxfp8_scale_byte(most);
-      const uint2 q = mxfp8_pack8(v[i], mx_inverse_scale(byte), byte == 255u);
+      const uint2 q = mxfp8_pack8(y, mx_inverse_scale(byte), byte == 255u);
       uint8_t* o = out + row * k + at;
       if constexpr (kAligned) {
         *reinterpret_cast<uint2*>(o) = q;

@@ -140,8 +140,8 @@ def rmsnorm_mxfp8_quant(
     127). The scale is the least power of two with which no value of its block
     saturates; a block that holds a NaN or an infinity is NaN throughout (scale
     255). ``input`` is bf16, fp16 or fp32 with K a multiple of 32 up to 65536; a
-    two-dimensional ``input`` may have strided rows. The scales come from the
-    32-bit norm itself, which is never rounded on the way."""
+    two-dimensional ``input`` may have strided rows. The scales are
+    those of the unrounded norm, held in 64 bits next to the border of two."""
     return get_ext().mx_quant(input, None, weight, out, out_scale, eps)
 
 

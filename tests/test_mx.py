@@ -382,6 +382,25 @@ def test_norm(rows, k, dtype, add):
 
 
 @gpu
+@pytest.mark.parametrize("k", [128, 4096])
+def test_norm_next_to_the_border_of_two_scales(k):
+    """Values within 3 steps of 1.75, where the scale changes: roundings of 32 bits
+    on the way reach as far, and the scale is that of 64 bits all the same."""
+    import flashinfer_amd as fi
+
+    torch.manual_seed(k)
+    x = (torch.rand(512, 1, device="cuda") * 1000 + 1000).expand(512, k).contiguous()
+    step = torch.arange(k // BLOCK, device="cuda") % 7 - 3
+    w = (1.75 + step * 2.0 ** -23).float().repeat_interleave(BLOCK)
+    q, s = fi.rmsnorm_mxfp8_quant(x, w)
+    # eps takes 1e-13 to 5e-13 away, far more than 64 bits round
+    y = norm64(x, w, 1e-6)[:, ::BLOCK]
+    assert torch.equal(s, torch.where(y > 1.75, 120, 119).to(torch.uint8))
+    # four blocks hold the steps -3 to 0 alone
+    assert bool((y < 1.75).any()) and bool((y > 1.75).any()) == (k > 128)
+
+
+@gpu
 def test_norm_of_zero_and_unlike_rows():
     import flashinfer_amd as fi
 
