@@ -682,12 +682,13 @@ def test_results_repeat_bit_by_bit(m, n, k, kind):
 
 
 @gpu
-def test_rows_too_far_apart_for_32_bits():
+@pytest.mark.parametrize("m", [40, 70])
+def test_rows_too_far_apart_for_32_bits(m):
     """A tile counts bytes in 32 bits; rows 16 MB apart do not fit it."""
     import flashinfer_amd as fi
 
     torch.manual_seed(0)
-    m, n, k = 40, 96, 256
+    n, k = 96, 256
     wide = torch.zeros(m, (1 << 23) + 8, dtype=torch.bfloat16, device="cuda")
     wide[:, :k] = torch.randn(m, k, device="cuda")
     b, b_scale = weights4(n, k)
