@@ -8,7 +8,7 @@ namespace mx4 {
 // What a tile costs: us to start and to finish, and us for 1024 of K where a CU
 // holds one workgroup and where it holds two. Fitted to K = 1024, 2048 and 7680
 // with 256, 512 and 1024 tiles (each time within 17 %; 25 % for 128 x 32); the
-// tile chosen is within 2 % of the best one over random products. Large tiles
+// tile chosen is within 2 to 3 % of the best one over random products. Large tiles
 // move fewer bytes for a product, small ones leave fewer CUs without work.
 // `apart`: how much longer it takes where rows of a do not start at multiples of
 // 128 bytes, so that every piece of one lies in two lines (K = 2080 to 7680).
@@ -30,10 +30,10 @@ constexpr Cost kCosts8[] = {
     {k128x32x4, 128, 32, 1.3f, 2.2f, 0.f, 1.33f},
 };
 
-// 8 bits in and out, where the small tiles widen their operands
+// 8 bits in and out, where every tile widens its operands (worst fit 15 %)
 constexpr Cost kCosts8to8[] = {
-    {k256x128, 256, 128, 3.6f, 8.6f, 14.7f, 1.26f}, {k128x128, 128, 128, 2.2f, 4.6f, 8.1f, 1.16f},
-    {k128x128x2, 128, 128, 3.2f, 4.2f, 0.f, 1.27f}, {k128x64, 128, 64, 2.1f, 3.7f, 0.f, 1.25f},
+    {k256x128, 256, 128, 4.1f, 13.f, 24.f, 1.11f},  {k128x128, 128, 128, 1.4f, 7.9f, 13.9f, 1.14f},
+    {k128x128x2, 128, 128, 2.5f, 6.9f, 0.f, 1.15f}, {k128x64, 128, 64, 2.1f, 3.7f, 0.f, 1.25f},
     {k64x64x4, 64, 64, 1.7f, 2.1f, 0.f, 1.28f},     {k64x32x4, 64, 32, 0.8f, 1.6f, 0.f, 1.22f},
     {k128x32x4, 128, 32, 1.3f, 2.4f, 0.f, 1.33f},
 };
@@ -89,8 +89,7 @@ Plan make_plan(int M, int N, int K, bool gated, bool act8, bool out8) {
               (f.start2 + f.two * k);
   }
   const Cost* costs = !act8 ? kCosts16 : out8 ? kCosts8to8 : kCosts8;
-  // the first three tiles do not widen 8-bit operands
-  for (int i = act8 && out8 && M <= 128 ? 3 : 0; i < 7; ++i) {
+  for (int i = 0; i < 7; ++i) {
     const Cost& c = costs[i];
     const int64_t tiles = ceil_div64(rows, c.rows) * ceil_div64(M, c.tokens);
     for (int parts = 1; parts <= kMostParts && parts <= loads; ++parts) {
