@@ -164,19 +164,23 @@ __device__ __forceinline__ bool f16_exact(uint32_t byte) {
 // In assembly, for the compiler holds every read of shared memory behind such
 // a load, also where the two go to different buffers: with the builtin the
 // next step's loads were waited for before this step's products. Nothing waits
-// for it here: the callers count these loads.
+// for it here: the callers count these loads. m0 is the compiler's own register,
+// of which it warns; that it is written has to be said all the same.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void load_lds16(const uint8_t* src, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off"
                :
                : "s"(dst), "v"(src)
-               : "memory");
+               : "memory", "m0");
 }
 __device__ __forceinline__ void load_lds16(const uint8_t* base, uint32_t at, uint32_t dst) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
                :
                : "s"(dst), "v"(at), "s"(base)
-               : "memory");
+               : "memory", "m0");
 }
+#pragma clang diagnostic pop
 
 __device__ __forceinline__ uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) void*)p;

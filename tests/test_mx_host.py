@@ -1,0 +1,26 @@
+"""What the MX operators do ahead of a launch, and what their sources promise the
+compiler: no GPU is needed for any of it."""
+import re
+from pathlib import Path
+
+import pytest
+import torch
+
+import flashinfer_amd
+from flashinfer_amd._lib import has_ext
+
+CSRC = Path(flashinfer_amd.__file__).parent / "csrc"
+needs_ext = pytest.mark.skipif(not has_ext(), reason="native extension not built")
+
+
+def asm_statements():
+    for path in sorted([*CSRC.rglob("*.hip"), *CSRC.rglob("*.hpp")]):
+        for found in re.finditer(r"\basm\b[^;]*?\((.*?)\);", path.read_text(), re.S):
+            yield path.name, found.group(1)
+
+
+def test_assembly_that_writes_m0_says_so():
+    writers = [(name, text) for name, text in asm_statements() if re.search(r"\bs_mov_b32 m0\b", text)]
+    assert len(writers) >= 2
+    for name, text in writers:
+        assert '"m0"' in text.rsplit(":", 1)[-1], f"{name}: {text}"
