@@ -1024,6 +1024,24 @@ std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tens
   return {q, s};
 }
 
+// The three entries name what each of them needs: without its weight or its
+// residual a call is refused by its signature rather than computed as another one.
+std::tuple<at::Tensor, at::Tensor> mxfp8_quantize(at::Tensor x, c10::optional<at::Tensor> out,
+                                                  c10::optional<at::Tensor> out_scale) {
+  return mx_quant(x, c10::nullopt, c10::nullopt, out, out_scale, 0.0);
+}
+std::tuple<at::Tensor, at::Tensor> mxfp8_rmsnorm(at::Tensor x, at::Tensor w,
+                                                 c10::optional<at::Tensor> out,
+                                                 c10::optional<at::Tensor> out_scale, double eps) {
+  return mx_quant(x, c10::nullopt, w, out, out_scale, eps);
+}
+std::tuple<at::Tensor, at::Tensor> mxfp8_add_rmsnorm(at::Tensor x, at::Tensor residual,
+                                                     at::Tensor w, c10::optional<at::Tensor> out,
+                                                     c10::optional<at::Tensor> out_scale,
+                                                     double eps) {
+  return mx_quant(x, residual, w, out, out_scale, eps);
+}
+
 int mx_type(at::ScalarType t) {
   return t == at::kBFloat16 ? 0 : t == at::kHalf ? 1 : t == at::kFloat8_e4m3fn ? 2 : -1;
 }
@@ -1512,7 +1530,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("chain_speculative", &chain_speculative_op);
   m.def("mla_run", &mla_run);
   m.def("group_gemm_nt", &group_gemm_nt);
-  m.def("mx_quant", &mx_quant);
+  m.def("mxfp8_quantize", &mxfp8_quantize);
+  m.def("mxfp8_rmsnorm", &mxfp8_rmsnorm);
+  m.def("mxfp8_add_rmsnorm", &mxfp8_add_rmsnorm);
   m.def("gemm_mxfp4_nt", &gemm_mxfp4_nt);
   m.def("gemm_mxfp4_nt_gated", &gemm_mxfp4_nt_gated);
   m.def("gemm_fp8_grouped", &gemm_fp8_grouped);

@@ -41,7 +41,7 @@ def mxfp8_quantize(
     its block saturates; a block that holds a NaN or an infinity is NaN throughout
     (scale 255). What :func:`flashinfer_amd.gemm_mxfp4_nt` takes as ``a`` and
     ``a_scale``."""
-    return get_ext().mx_quant(x, None, None, out, out_scale, 0.0)
+    return get_ext().mxfp8_quantize(x, out, out_scale)
 
 
 def per_block_quant_mxfp8(

@@ -142,7 +142,7 @@ def rmsnorm_mxfp8_quant(
     255). ``input`` is bf16, fp16 or fp32 with K a multiple of 32 up to 65536; a
     two-dimensional ``input`` may have strided rows. The scales are
     those of the unrounded norm, held in 64 bits next to the border of two."""
-    return get_ext().mx_quant(input, None, weight, out, out_scale, eps)
+    return get_ext().mxfp8_rmsnorm(input, weight, out, out_scale, eps)
 
 
 @flashinfer_api
@@ -158,7 +158,7 @@ def fused_add_rmsnorm_mxfp8_quant(
     r"""In place ``residual += input``, then the RMSNorm of the residual as it is
     stored, written as MXFP8: returns ``(out, out_scale)`` as
     :func:`rmsnorm_mxfp8_quant` does."""
-    return get_ext().mx_quant(input, residual, weight, out, out_scale, eps)
+    return get_ext().mxfp8_add_rmsnorm(input, residual, weight, out, out_scale, eps)
 
 
 @flashinfer_api

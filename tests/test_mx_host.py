@@ -24,3 +24,17 @@ def test_assembly_that_writes_m0_says_so():
     assert len(writers) >= 2
     for name, text in writers:
         assert '"m0"' in text.rsplit(":", 1)[-1], f"{name}: {text}"
+
+
+@needs_ext
+@pytest.mark.parametrize("call", [
+    lambda fi, x, w: fi.rmsnorm_mxfp8_quant(x, None),
+    lambda fi, x, w: fi.fused_add_rmsnorm_mxfp8_quant(x, x.clone(), None),
+    lambda fi, x, w: fi.fused_add_rmsnorm_mxfp8_quant(x, None, w),
+    lambda fi, x, w: fi.mxfp8_quantize(None),
+])
+def test_a_missing_operand_is_refused(call):
+    """Without its weight a norm would be a quantization, and without its residual
+    an addition would be left out."""
+    with pytest.raises(TypeError, match="incompatible function arguments"):
+        call(flashinfer_amd, torch.zeros(2, 64), torch.zeros(64))
