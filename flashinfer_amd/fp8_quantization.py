@@ -9,6 +9,8 @@ from typing import Optional, Tuple
 import torch
 
 from ._lib import get_ext
+from .api_logging import flashinfer_api
+from .fi_trace import fi_trace
 from .utils import ceil_div
 
 _FP8 = torch.float8_e4m3fn
@@ -30,6 +32,8 @@ def per_token_group_quant_fp8(
     return q.view(_FP8), scale
 
 
+@flashinfer_api
+@fi_trace
 def mxfp8_quantize(
     x: torch.Tensor, out: Optional[torch.Tensor] = None,
     out_scale: Optional[torch.Tensor] = None,

@@ -21,6 +21,8 @@ MX_BLOCK = 32
 _ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2}
 
 
+@flashinfer_api
+@fi_trace
 def mxfp4_quantize(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     r"""Weights ``[..., N, K]`` as MXFP4: ``(b [..., N, K // 2], b_scale [..., N,
     K // 32])``, both uint8. The scale is the least power of two with which no

@@ -38,3 +38,33 @@ def test_a_missing_operand_is_refused(call):
     an addition would be left out."""
     with pytest.raises(TypeError, match="incompatible function arguments"):
         call(flashinfer_amd, torch.zeros(2, 64), torch.zeros(64))
+
+
+ENTRIES = ["rmsnorm_mxfp8_quant", "fused_add_rmsnorm_mxfp8_quant", "mxfp8_quantize", "mxfp4_quantize",
+           "gemm_mxfp4_nt", "gemm_mxfp4_nt_gated"]
+
+
+@pytest.mark.parametrize("name", ENTRIES)
+def test_a_substitute_takes_over_every_entry(name):
+    from flashinfer_amd import trace_apply
+
+    trace_apply.enable_apply({name: lambda *args, **kw: (name, args, kw)})
+    try:
+        assert getattr(flashinfer_amd, name)(1, out=2) == (name, (1,), {"out": 2})
+    finally:
+        trace_apply.disable_apply()
+
+
+def test_every_entry_is_logged():
+    import os
+    import subprocess
+    import sys
+
+    code = ("import flashinfer_amd as fi\n"
+            f"for name in {ENTRIES}:\n"
+            "    try: getattr(fi, name)(None)\n"
+            "    except Exception: pass\n")
+    run = subprocess.run([sys.executable, "-c", code], env={**os.environ, "FLASHINFER_LOGLEVEL": "1"},
+                         cwd=CSRC.parent.parent, capture_output=True, text=True, check=True)
+    for name in ENTRIES:
+        assert f"[flashinfer_amd] {name}" in run.stderr.splitlines()
