@@ -43,7 +43,11 @@ def mxfp4_quantize(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     exponent = (exponent - 3 + (mantissa > 0.75)).clamp(-127, 127)
     bad = ~torch.isfinite(most)
     exponent = torch.where(bad | (most == 0), torch.zeros_like(exponent), exponent)
-    scaled = torch.ldexp(blocks, -exponent.unsqueeze(-1))
+    # 2^-exponent from its bits: on a GPU torch.ldexp takes a power that is off by a
+    # step for some exponents, and the middle of two levels is no longer met. The
+    # largest exponent is 126.
+    inverse = ((127 - exponent) << 23).view(torch.float32)
+    scaled = blocks * inverse.unsqueeze(-1)
     a = scaled.abs()
     # codes 0..7 are 0, .5, 1, 1.5, 2, 3, 4, 6; the middle of two neighbours
     # goes to the even code: up from an odd code, down from an even one

@@ -68,3 +68,19 @@ def test_every_entry_is_logged():
                          cwd=CSRC.parent.parent, capture_output=True, text=True, check=True)
     for name in ENTRIES:
         assert f"[flashinfer_amd] {name}" in run.stderr.splitlines()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_mxfp4_quantize_on_the_gpu_is_that_of_the_cpu(dtype):
+    gen = torch.Generator().manual_seed(0)
+    top = 15 if dtype == torch.float16 else 126
+    w = torch.randint(-16, 17, (3, 512, 96), generator=gen).double() / 4  # ties among them
+    w += torch.randn(w.shape, generator=gen) * (torch.rand(w.shape, generator=gen) < 0.5)
+    w *= torch.exp2(torch.randint(-top - 12, top - 3, (3, 512, 3), generator=gen).double()
+                    ).repeat_interleave(32, -1)
+    w = w.to(dtype)
+    w[0, 0, 3], w[0, 1, 40], w[0, 2] = float("nan"), float("inf"), 0
+    b, s = flashinfer_amd.mxfp4_quantize(w)
+    got_b, got_s = flashinfer_amd.mxfp4_quantize(w.cuda())
+    assert torch.equal(got_s.cpu(), s) and torch.equal(got_b.cpu(), b)
