@@ -27,8 +27,8 @@ def mxfp4_quantize(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     r"""Weights ``[..., N, K]`` as MXFP4: ``(b [..., N, K // 2], b_scale [..., N,
     K // 32])``, both uint8. The scale is the least power of two with which no
     value of its block saturates; values round to the nearest, ties to the one
-    with an even code. A block that holds a NaN or an infinity becomes NaN (scale
-    255). Done once when weights are loaded."""
+    with an even code. A block that holds a NaN, an infinity or more than 6 * 2^127
+    becomes NaN (scale 255). Done once when weights are loaded."""
     if w.dim() < 2 or w.shape[-1] == 0 or w.shape[-1] % MX_BLOCK:
         raise ValueError(
             f"mxfp4_quantize needs [..., N, K] with K a multiple of {MX_BLOCK}, "
@@ -36,17 +36,22 @@ def mxfp4_quantize(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
         )
     if not w.dtype.is_floating_point:
         raise ValueError(f"mxfp4_quantize needs a floating type, got {w.dtype}")
-    blocks = w.float().unflatten(-1, (-1, MX_BLOCK))
+    # float64 stays: rounded to 32 bits first, a value next to the middle of two
+    # levels could go to the wrong one
+    wide = w if w.dtype == torch.float64 else w.float()
+    blocks = wide.unflatten(-1, (-1, MX_BLOCK))
     most = blocks.abs().amax(-1)
     mantissa, exponent = torch.frexp(most)
     # most = mantissa * 2^exponent with mantissa in [.5, 1), and 6 = .75 * 2^3
     exponent = (exponent - 3 + (mantissa > 0.75)).clamp(-127, 127)
-    bad = ~torch.isfinite(most)
+    bad = ~(most.double() <= 6.0 * 2.0 ** 127)  # a NaN too
     exponent = torch.where(bad | (most == 0), torch.zeros_like(exponent), exponent)
     # 2^-exponent from its bits: on a GPU torch.ldexp takes a power that is off by a
-    # step for some exponents, and the middle of two levels is no longer met. The
-    # largest exponent is 126.
-    inverse = ((127 - exponent) << 23).view(torch.float32)
+    # step for some exponents, and the middle of two levels is no longer met
+    if wide.dtype == torch.float64:
+        inverse = ((1023 - exponent.long()) << 52).view(torch.float64)
+    else:  # 126 is the largest exponent here
+        inverse = ((127 - exponent) << 23).view(torch.float32)
     scaled = blocks * inverse.unsqueeze(-1)
     a = scaled.abs()
     # codes 0..7 are 0, .5, 1, 1.5, 2, 3, 4, 6; the middle of two neighbours

@@ -70,8 +70,24 @@ def test_every_entry_is_logged():
         assert f"[flashinfer_amd] {name}" in run.stderr.splitlines()
 
 
+def test_mxfp4_quantize_takes_64_bits_as_they_are():
+    from test_mx import from4
+
+    w = torch.zeros(4, 32, dtype=torch.float64)
+    w[0, :5] = torch.tensor([6, 0.25, 1.25, 2.5, 5], dtype=torch.float64) * (1 + 2.0 ** -40)
+    w[0, 0] = 6                   # a step above the middles of two levels: not ties
+    w[1, 0] = 6 * (1 + 2.0 ** -40)  # saturates by a little at the scale of 1
+    w[2, 0] = 6 * 2.0 ** 127      # no float32, but the largest value of the format
+    w[3, 0] = 6 * 2.0 ** 127 * (1 + 2.0 ** -40)
+    b, s = flashinfer_amd.mxfp4_quantize(w)
+    d = from4(b, s)
+    assert torch.equal(d[0, :5], torch.tensor([6, 0.5, 1.5, 3, 6], dtype=torch.float64))
+    assert s[1, 0] == 128 and s[2, 0] == 254 and d[2, 0] == w[2, 0]
+    assert s[3, 0] == 255 and d[3].isnan().all()
+
+
 @pytest.mark.gpu
-@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32, torch.float64])
 def test_mxfp4_quantize_on_the_gpu_is_that_of_the_cpu(dtype):
     gen = torch.Generator().manual_seed(0)
     top = 15 if dtype == torch.float16 else 126
