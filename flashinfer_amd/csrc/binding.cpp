@@ -91,7 +91,7 @@ hipError_t fi_gemm_fp8_grouped(const void* A, const void* W, void* C,
                                float scalar_scale, int64_t a_scale_stride,
                                int flat_tiles, int mx, hipStream_t stream);
 hipError_t fi_mx_quant(int dtype, const void* x, void* residual, const void* w, void* out,
-                       void* scale, int rows, int k, int64_t sx, int64_t sr, float eps,
+                       void* scale, int rows, int k, int64_t sx, int64_t sr, double eps,
                        int aligned, hipStream_t stream);
 hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act, const void* a,
                          const void* a_scale, const void* b, const void* b_scale,
@@ -1019,7 +1019,7 @@ std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tens
                        reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0;
   check_hip(fi_mx_quant(dtype_code(x), x.data_ptr(), r ? r->data_ptr() : nullptr,
                         wp ? wp->data_ptr() : nullptr, q.data_ptr(), s.data_ptr(), (int)rows,
-                        (int)K, sx, sr, (float)eps, aligned, cur_stream(x)),
+                        (int)K, sx, sr, eps, aligned, cur_stream(x)),
             "fi_mx_quant");
   return {q, s};
 }

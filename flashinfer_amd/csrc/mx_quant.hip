@@ -39,7 +39,7 @@ template <typename T, int NV, bool kNorm, bool kAdd, bool kAligned>
 __global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
     const T* __restrict__ x, T* __restrict__ residual, const T* __restrict__ w,
     uint8_t* __restrict__ out, uint8_t* __restrict__ scale, int rows, int k, int64_t stride_x,
-    int64_t stride_r, float eps, int lanes) {
+    int64_t stride_r, double eps, int lanes) {
   constexpr bool kShort = NV == 0;
   constexpr int kGroups = kShort ? 1 : NV;
   __shared__ double sums[16];
@@ -94,7 +94,7 @@ __global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
       ss = 0.;
       for (int i = 0; i < waves; ++i) ss += sums[i];
     }
-    rrms = 1. / sqrt(ss / k + (double)eps);
+    rrms = 1. / sqrt(ss / k + eps);
   }
 #pragma unroll
   for (int i = 0; i < kGroups; ++i) {
@@ -141,7 +141,7 @@ __global__ __launch_bounds__(NV ? 1024 : 256) void mx_quant_kernel(
 
 template <typename T, bool kNorm, bool kAdd, bool kAligned>
 hipError_t launch(const void* x, void* residual, const void* w, void* out, void* scale,
-                  int rows, int k, int64_t sx, int64_t sr, float eps, hipStream_t stream) {
+                  int rows, int k, int64_t sx, int64_t sr, double eps, hipStream_t stream) {
   // Two groups to a lane from 4096 values on: 512 lanes with two wait for their
   // sum with half the waves of 1024 with one (16384 x 8192: 5.7 and 5.45 TB/s,
   // 4096 x 7168: 5.6 and 5.2), and 896 lanes with two beat 448 with four
@@ -183,7 +183,7 @@ hipError_t launch(const void* x, void* residual, const void* w, void* out, void*
 
 template <typename T>
 hipError_t dispatch(const void* x, void* residual, const void* w, void* out, void* scale,
-                    int rows, int k, int64_t sx, int64_t sr, float eps, int aligned,
+                    int rows, int k, int64_t sx, int64_t sr, double eps, int aligned,
                     hipStream_t stream) {
 #define FI_GO(NORM, ADD)                                                                  \
   (aligned ? launch<T, NORM, ADD, true>(x, residual, w, out, scale, rows, k, sx, sr, eps, \
@@ -204,7 +204,7 @@ hipError_t dispatch(const void* x, void* residual, const void* w, void* out, voi
 // out starts at a multiple of 8.
 extern "C" hipError_t fi_mx_quant(int dtype, const void* x, void* residual, const void* w,
                                   void* out, void* scale, int rows, int k, int64_t sx,
-                                  int64_t sr, float eps, int aligned, hipStream_t stream) {
+                                  int64_t sr, double eps, int aligned, hipStream_t stream) {
   if (rows == 0) return hipSuccess;
   if (k <= 0 || k % fi::kMxBlock != 0 || k > 65536) return hipErrorInvalidValue;
   switch (dtype) {

@@ -84,3 +84,28 @@ def test_16_bit_products_are_those_of_32_bit_sums(m, n, k, kind):
     want = (a64 @ w64.T).to(a.dtype)
     assert want.isfinite().all()
     assert torch.equal(fi.gemm_mxfp4_nt(a, b, b_scale), want)
+
+
+@gpu
+def test_norm_takes_eps_in_64_bits():
+    """0.1 is no float32: rounded to one it is off by 1.5e-8, enough to take a value
+    next to the border of two scales over it."""
+    import flashinfer_amd as fi
+
+    from test_mx import norm64
+
+    eps = 0.1
+    w = (100 * (1 + torch.arange(64, device="cuda") * 2.0 ** -20)).float().repeat_interleave(BLOCK)
+    # where 100 c / sqrt(c^2 + eps) is 1.75, and a thousand steps around it
+    middle = 1.75 * (eps / (100 ** 2 - 1.75 ** 2)) ** 0.5
+    start = torch.tensor(middle, device="cuda").view(torch.int32) - 1600
+    c = (start + torch.arange(2048, dtype=torch.int32, device="cuda")).view(torch.float32)
+    x = c[:, None].expand(2048, 2048).contiguous()
+    _, s = fi.rmsnorm_mxfp8_quant(x, w, eps=eps)
+
+    def scales(e):
+        return torch.where(norm64(x, w, e)[:, ::BLOCK] > 1.75, 120, 119).to(torch.uint8)
+
+    want = scales(eps)
+    assert not torch.equal(want, scales(torch.tensor(eps).item())), "no value that eps decides"
+    assert torch.equal(s, want)
