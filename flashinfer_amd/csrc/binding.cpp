@@ -98,6 +98,8 @@ hipError_t fi_gemm_mxfp4(int a_type, int out_type, int gated, int act, const voi
                          void* out, void* out_scale, float* floats, int M, int N, int K,
                          int64_t lda, int64_t ldo, hipStream_t stream);
 int64_t fi_gemm_mxfp4_floats(int a_type, int out_type, int gated, int M, int N, int K);
+const char* fi_gemm_mxfp4_plan(int a_type, int out_type, int gated, int M, int N, int K,
+                               int* parts);
 hipError_t fi_per_group_quant_fp8(int dtype, int trans_scale, const void* x, void* q,
                                   float* scale, int64_t rows, int K, int64_t stride_row,
                                   float eps, hipStream_t stream);
@@ -1171,6 +1173,14 @@ std::tuple<at::Tensor, c10::optional<at::Tensor>> gemm_mxfp4_nt_gated(
                        out_dtype);
 }
 
+// (kernel, parts of K) of a product: what the tests hold their sizes against
+std::tuple<std::string, int> gemm_mxfp4_plan(at::ScalarType a, at::ScalarType out, bool gated,
+                                             int M, int N, int K) {
+  int parts = 1;
+  const std::string name = fi_gemm_mxfp4_plan(mx_type(a), mx_type(out), gated, M, N, K, &parts);
+  return {name, parts};
+}
+
 // per-128-group fp8 quantization: returns (q uint8 [rows,K], scale f32)
 void per_group_quant_fp8(at::Tensor x, at::Tensor q, at::Tensor scale,
                          bool trans_scale, double eps) {
@@ -1535,6 +1545,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("mxfp8_add_rmsnorm", &mxfp8_add_rmsnorm);
   m.def("gemm_mxfp4_nt", &gemm_mxfp4_nt);
   m.def("gemm_mxfp4_nt_gated", &gemm_mxfp4_nt_gated);
+  m.def("gemm_mxfp4_plan", &gemm_mxfp4_plan);
   m.def("gemm_fp8_grouped", &gemm_fp8_grouped);
   m.def("per_group_quant_fp8", &per_group_quant_fp8);
   m.def("scale_quant_fp8", &scale_quant_fp8);

@@ -119,6 +119,24 @@ extern "C" int64_t fi_gemm_mxfp4_floats(int a_type, int out_type, int gated, int
   return make_plan(M, N, K, gated, a_type == kFp8, out_type == kFp8).floats;
 }
 
+// Which kernel this product gets, and in how many parts of K over workgroups.
+extern "C" const char* fi_gemm_mxfp4_plan(int a_type, int out_type, int gated, int M, int N,
+                                          int K, int* parts) {
+  using namespace fi::mx4;
+  const Plan plan = make_plan(M, N, K, gated, a_type == kFp8, out_type == kFp8);
+  *parts = plan.parts;
+  switch (plan.shape) {
+    case k256x128: return "256x128";
+    case k128x128: return "128x128";
+    case k128x128x2: return "128x128x2";
+    case k128x64: return "128x64";
+    case k64x64x4: return "64x64x4";
+    case k64x32x4: return "64x32x4";
+    case k128x32x4: return "128x32x4";
+  }
+  return "rows";
+}
+
 // a_type: 0 bf16, 1 fp16, 2 e4m3 with scale bytes; out_type the same, 2 for the
 // gated form alone and N a multiple of 32. N counts outputs; the gated form
 // reads 2 * N weight rows. act: 0 silu, 1 gelu, 2 gelu with tanh. K is a

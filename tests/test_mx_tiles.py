@@ -1,0 +1,101 @@
+"""Every kernel that an MXFP4 product can get, whole and in parts of K: the sizes
+below reach each of them for each type and form, which a test without a GPU holds
+against the choice itself."""
+import math
+import random
+
+import pytest
+import torch
+
+from flashinfer_amd._lib import get_ext, has_ext
+from test_mx import (FP8, OUT_HALF, act64, activations, from4, gpu, product_off, to8_bits, weights4)
+from test_mx_sums import exact_tokens, exact_weights
+
+BF16 = torch.bfloat16
+# type of a, of the output, gated
+FORMS = {"16 bits": (BF16, BF16, False), "MXFP8": (FP8, BF16, False),
+         "gated, 16 bits": (BF16, BF16, True), "gated, 16 bits to MXFP8": (BF16, FP8, True),
+         "gated, MXFP8 to 16 bits": (FP8, BF16, True), "gated, MXFP8": (FP8, FP8, True)}
+PLAIN = [(1, 33, 32), (34, 33, 32), (65, 37, 2752), (4164, 67, 32), (20, 16905, 32), (34, 17448, 32),
+         (67, 16830, 32), (261, 22424, 32), (2093, 33, 7072), (65, 18853, 480), (92, 2066, 7360),
+         (4828, 77, 6112), (2889, 74, 11360), (4244, 92, 14240), (5577, 340, 7584), (215, 17423, 13728),
+         (66, 16961, 3200), (342, 3170, 13184), (223, 10402, 8960), (1788, 2434, 13248)]
+GATED = [(1, 32, 32), (81, 4192, 32), (33, 10400, 32), (65, 8544, 32), (40, 8800, 192), (72, 1440, 8352),
+         (65, 12256, 1120), (274, 17760, 288), (163, 1056, 11712), (255, 1056, 14176), (115, 8416, 8672),
+         (1925, 544, 9056), (71, 18144, 15200), (890, 2112, 4352), (2164, 1056, 9216), (4145, 96, 96),
+         (70, 96, 4128), (70, 96, 96), (260, 320, 6176), (100, 4256, 13056)]
+
+
+def chosen(form, m, n, k):
+    name, parts = get_ext().gemm_mxfp4_plan(*FORMS[form], m, n, k)
+    return name, parts > 1
+
+
+@pytest.mark.skipif(not has_ext(), reason="native extension not built")
+@pytest.mark.parametrize("form", FORMS)
+def test_the_sizes_reach_every_kernel(form):
+    rng = random.Random(0)
+
+    def size(most):
+        return round(math.exp(rng.uniform(0, math.log(most))))
+
+    reached = {chosen(form, size(8192), 32 * size(1024), 32 * size(512)) for _ in range(40000)}
+    assert len(reached) > 10
+    missing = reached - {chosen(form, *s) for s in (GATED if FORMS[form][2] else PLAIN)}
+    assert not missing, f"no size for {sorted(missing)}"
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", PLAIN)
+def test_plain(m, n, k, kind):
+    import flashinfer_amd as fi
+
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    if kind == "fp8":
+        a, a_scale, a64 = activations(m, k, kind, gen)
+        b, b_scale = weights4(n, k, gen)
+        w64 = from4(b, b_scale)
+        want, off = a64 @ w64.T, product_off(a64, w64, kind)
+        for dtype in (torch.bfloat16, torch.float16):
+            out = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale, out_dtype=dtype)
+            # fp16 has a least step of 2^-24
+            bound = off + OUT_HALF[dtype] * (want.abs() + off) + 2.0 ** -25
+            assert ((out.double() - want).abs() <= bound).all()
+    else:
+        a, a_scale, a64, at = exact_tokens(m, k, kind, gen)
+        b, b_scale, w64 = exact_weights(n, k, at, gen, positive=False)
+        want = a64 @ w64.T
+        for dtype in (torch.bfloat16, torch.float16):
+            assert torch.equal(fi.gemm_mxfp4_nt(a, b, b_scale, out_dtype=dtype), want.to(dtype))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", GATED)
+def test_gated(m, n, k, kind):
+    import flashinfer_amd as fi
+
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    a, a_scale, a64, at = exact_tokens(m, k, kind, gen)
+    b, b_scale, w64 = exact_weights(2 * n, k, at, gen, positive=True)
+    # silu(g) is g in 32 bits where exp(-g) vanishes beside 1
+    g, u = a64 @ w64[:n].T, a64 @ w64[n:].T
+    assert g.min() > 20 and max(g.max(), u.abs().max()) < 2 ** 22
+    y = (g * u).float()
+    want_q, want_s = to8_bits(y)
+    q, s = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=FP8)
+    assert torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q)
+    if kind != "fp8":
+        assert torch.equal(fi.gemm_mxfp4_nt_gated(a, b, b_scale, out_dtype=BF16), y.to(BF16))
+        return
+    a, a_scale, a64 = activations(m, k, kind, gen)
+    b, b_scale = weights4(2 * n, k, gen)
+    w64 = from4(b, b_scale)
+    g, u = a64 @ w64[:n].T, a64 @ w64[n:].T
+    og, ou = product_off(a64, w64[:n], kind), product_off(a64, w64[n:], kind)
+    want = act64(g, "silu") * u
+    og = 1.13 * og + 8 * 2.0 ** -24 * g.abs()
+    off = og * (u.abs() + ou) + act64(g, "silu").abs() * ou
+    out = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=BF16)
+    assert ((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
