@@ -99,3 +99,37 @@ def test_gated(m, n, k, kind):
     off = og * (u.abs() + ou) + act64(g, "silu").abs() * ou
     out = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=BF16)
     assert ((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m", [70, 97])
+def test_rows_too_far_apart_for_32_bits(m, kind):
+    """Rows 16 MB apart go 16 tokens at a time through the kernel for few tokens,
+    with their own scales, outputs and output scales; so do outputs far apart."""
+    import flashinfer_amd as fi
+
+    gen = torch.Generator(device="cuda").manual_seed(m)
+    n, k = 96, 288
+    a, a_scale, a64, at = exact_tokens(m, k, kind, gen)
+    b, b_scale, w64 = exact_weights(2 * n, k, at, gen, positive=True)
+    far = torch.empty(m, (1 << 24) // a.element_size() + 16, dtype=a.dtype, device="cuda")[:, :k]
+    far.copy_(a)
+    if kind == "fp8":
+        # scales of its own for every row, within what 32 bits add up exactly
+        a_scale += (torch.arange(m, device="cuda") % 5).to(torch.uint8)[:, None]
+        a64 = a64 * 2.0 ** (torch.arange(m, device="cuda") % 5)[:, None]
+    g, u = a64 @ w64[:n].T, a64 @ w64[n:].T
+    want_q, want_s = to8_bits((g * u).float())
+    assert len({tuple(r) for r in want_s.tolist()}) > 1
+    q, s = fi.gemm_mxfp4_nt_gated(far, b, b_scale, a_scale, out_dtype=FP8)
+    assert torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q)
+    box = torch.empty(m, n + 40, dtype=torch.uint8, device="cuda").view(FP8)[:, :n]
+    q, s = fi.gemm_mxfp4_nt_gated(far, b, b_scale, a_scale, out=box)
+    assert torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q)
+    out = fi.gemm_mxfp4_nt(far, b, b_scale, a_scale, out_dtype=BF16)
+    if kind == "fp8":
+        want, off = a64 @ w64.T, product_off(a64, w64, kind)
+        assert ((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
+    else:
+        assert torch.equal(out, (a64 @ w64.T).to(BF16))
