@@ -133,3 +133,42 @@ def test_rows_too_far_apart_for_32_bits(m, kind):
         assert ((out.double() - want).abs() <= off + 2.0 ** -8 * (want.abs() + off)).all()
     else:
         assert torch.equal(out, (a64 @ w64.T).to(BF16))
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", [(1, 64, 32), (7, 7008, 160), (12, 96, 6176), (30, 64, 288)] + GATED[1:])
+def test_special_values_and_mxfp8_outputs(m, n, k, kind):
+    """A NaN or an infinity makes the blocks NaN that it reaches and leaves the others
+    as they were, bit by bit."""
+    import flashinfer_amd as fi
+
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    a, a_scale, _, at = exact_tokens(m, k, kind, gen)
+    b, b_scale, _ = exact_weights(2 * n, k, at, gen, positive=True)
+
+    def run():
+        q, s = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=FP8)
+        return q.view(torch.uint8).unflatten(1, (-1, 32)), s
+
+    q0, s0 = run()
+    assert (s0 < 255).all()
+    bad = torch.zeros(m, n // 32, dtype=torch.bool, device="cuda")
+    gate, up, last = n // 2, n + n - 1, k // 32 - 1
+    b_scale[gate, last] = 255
+    b[up, :16] = 0  # NaN times zero
+    b_scale[up, 0] = 255
+    bad[:, gate // 32] = bad[:, -1] = True
+    if m > 2:
+        if kind == "fp8":
+            a_scale[m // 2, last] = 255
+            a_scale[m - 1, 0] = 255
+            a.view(torch.uint8)[m - 1, :32] = 0
+        else:
+            a[m // 2, k - 1] = math.nan
+            a[m - 1, 3] = math.inf
+        bad[m // 2] = bad[m - 1] = True
+    q, s = run()
+    assert torch.equal(s == 255, bad)
+    assert (q[bad] & 0x7F == 0x7F).all()
+    assert torch.equal(s[~bad], s0[~bad]) and torch.equal(q[~bad], q0[~bad])
