@@ -1163,17 +1163,29 @@ __global__ __launch_bounds__(256) void join_kernel(Params p, int tiles_n, int ti
 }
 
 template <int ACT, bool GATED, bool OUT8, int WN, int WM, int GN, int GM, int GK>
-hipError_t launch_tile(const Params& p, int parts, hipStream_t stream) {
+hipError_t launch_tile(const Params& all, int parts, hipStream_t stream) {
   using C = Tile<ACT, GATED, WN, WM, GN, GM, GK>;
-  const int64_t tiles_n = ceil_div(p.N, C::kOut), tiles_m = ceil_div(p.M, C::TM);
-  const int64_t joins = tiles_n * tiles_m * GN * GM * WN * WM / (GATED ? 2 : 1);
-  if (joins >= (int64_t)1 << 31) return hipErrorInvalidValue;
-  hipLaunchKernelGGL((tile_kernel<ACT, GATED, OUT8, WN, WM, GN, GM, GK>),
-                     dim3((unsigned)(tiles_n * tiles_m), parts), dim3(C::kLaunch), 0, stream, p,
-                     (int)tiles_n, (int)tiles_m);
-  if (parts > 1)
-    hipLaunchKernelGGL((join_kernel<GATED, OUT8, WN, WM, GN, GM, GK>), dim3((unsigned)joins), dim3(256), 0,
-                       stream, p, (int)tiles_n, (int)tiles_m, parts);
+  const int64_t tiles_n = ceil_div(all.N, C::kOut);
+  // A launch has less than 2^32 threads: more tiles go some rows of them at a time.
+  // (Parts of K are for few tiles.)
+  const int64_t most = (((int64_t)1 << 32) - 1) / C::kLaunch / tiles_n;
+  for (int64_t m = 0; m < all.M; m += most * C::TM) {
+    Params p = all;
+    p.a = (const char*)p.a + m * p.lda * (ACT == kFp8 ? 1 : 2);
+    if (ACT == kFp8) p.a_scale += m * (p.K / kMxBlock);
+    p.out = (char*)p.out + m * p.ldo * (OUT8 ? 1 : 2);
+    if (OUT8) p.out_scale += m * (p.N / kMxBlock);
+    p.M = (int)(all.M - m < most * C::TM ? all.M - m : most * C::TM);
+    const int64_t tiles_m = ceil_div(p.M, C::TM);
+    hipLaunchKernelGGL((tile_kernel<ACT, GATED, OUT8, WN, WM, GN, GM, GK>),
+                       dim3((unsigned)(tiles_n * tiles_m), parts), dim3(C::kLaunch), 0, stream, p,
+                       (int)tiles_n, (int)tiles_m);
+    if (parts > 1) {
+      const int64_t joins = tiles_n * tiles_m * GN * GM * WN * WM / (GATED ? 2 : 1);
+      hipLaunchKernelGGL((join_kernel<GATED, OUT8, WN, WM, GN, GM, GK>), dim3((unsigned)joins),
+                         dim3(256), 0, stream, p, (int)tiles_n, (int)tiles_m, parts);
+    }
+  }
   return hipGetLastError();
 }
 

@@ -172,3 +172,27 @@ def test_special_values_and_mxfp8_outputs(m, n, k, kind):
     assert torch.equal(s == 255, bad)
     assert (q[bad] & 0x7F == 0x7F).all()
     assert torch.equal(s[~bad], s0[~bad]) and torch.equal(q[~bad], q0[~bad])
+
+
+@gpu
+def test_more_tiles_than_one_launch():
+    """Tiles of more than 2^32 threads: 547 x 32768 of 128 x 128 with 256 lanes each."""
+    import flashinfer_amd as fi
+
+    torch.cuda.empty_cache()
+    m, n, k = 70000, 2 ** 21, 32
+    assert chosen("gated, MXFP8", m, n, k) == ("128x128", False)
+    gen = torch.Generator(device="cuda").manual_seed(0)
+    a, a_scale, _, at = exact_tokens(m, k, "fp8", gen)
+    few, few_scale, _ = exact_weights(64, k, at, gen, positive=True)
+    b = torch.zeros(2 * n, k // 2, dtype=torch.uint8, device="cuda")
+    b_scale = torch.full((2 * n, k // 32), 127, dtype=torch.uint8, device="cuda")
+    b[n - 32:n], b[-32:] = few[:32], few[32:]
+    want_q, want_s = fi.gemm_mxfp4_nt_gated(a, few, few_scale, a_scale, out_dtype=FP8)
+    q, s = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=FP8)
+    assert torch.equal(s[:, -1:], want_s) and not s[:, :-1].any()
+    assert torch.equal(q[:, -32:].view(torch.uint8), want_q.view(torch.uint8))
+    for at in range(0, m, 10000):
+        assert not q[at:at + 10000, :-32].view(torch.uint8).any()
+    del q, s
+    torch.cuda.empty_cache()
