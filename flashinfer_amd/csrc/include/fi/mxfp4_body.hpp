@@ -13,8 +13,9 @@
 //     registers and 64+16g.. in the last four, its fp4 operand k = 32g..32g+31,
 //     and lane group g supplies the scale of block g for either.
 //   16-bit a: the block becomes bf16 (two values an instruction, the scale
-//     applied by it, exact for every scale) and feeds four 16x16x32 products;
-//     product i takes k = 32g + 8i .. 32g + 8i + 7 from lane group g.
+//     applied by it, exact below 2^128: 4 and 6 times 2^126, and 2 to 6 times
+//     2^127, become infinite) and feeds four 16x16x32 products; product i takes
+//     k = 32g + 8i .. 32g + 8i + 7 from lane group g.
 //   fp16 a: the same in fp16 where every scale of the wave's chunk keeps the
 //     weights exact in fp16 (2^-23 .. 2^13); elsewhere a is split into two
 //     bf16 parts, high and low, which hold its 11 bits exactly (a tile of many
@@ -24,8 +25,8 @@
 // of the magnitudes that a sum is made of, about 1e-5 of the result on normal data.
 // An output in 16 bits rounds to 4e-3 or 5e-4 and hides that. An MXFP8 output has
 // scales, and one block in 50,000 would get the neighbour of its own: there, for
-// any number of tokens, both operands become bf16 (an exact step) and the error is
-// that of 32 bits. Where the matrix unit bounds the time it costs the rate of 8-bit
+// any number of tokens, both operands become bf16 (exactly, from 2^-133 to below
+// 2^128) and the error is that of 32 bits. Where the matrix unit bounds the time it costs the rate of 8-bit
 // products (gated 4096 x 4096 x 7680: 377 us for 233).
 #pragma once
 #include <type_traits>

@@ -109,3 +109,98 @@ def test_norm_takes_eps_in_64_bits():
     want = scales(eps)
     assert not torch.equal(want, scales(torch.tensor(eps).item())), "no value that eps decides"
     assert torch.equal(s, want)
+
+
+def power64(e):
+    """2^e in 64 bits from its bits (torch.ldexp takes a power of 32, and a GPU's is
+    not always exact)."""
+    return ((e.long() + 1023) << 52).view(torch.float64)
+
+
+def scale_operands(m, n, k, kind):
+    """Tokens and weights of every size: row i of b has the scale byte 254 * i // (n - 1),
+    token i is about as large as the inverse of byte 254 * i // (m - 1)."""
+    gen = torch.Generator(device="cuda").manual_seed(m + n + k)
+    b_byte = torch.arange(n, device="cuda") * 254 // (n - 1)
+    code = torch.randint(1, 8, (n, k), device="cuda", generator=gen)
+    code[b_byte == 253] = code[b_byte == 253].clamp(max=5)  # 3: 4 * 2^126 is no float32
+    code[b_byte == 254] = code[b_byte == 254].clamp(max=3)  # 1.5
+    b = (code[:, 0::2] | code[:, 1::2] << 4).to(torch.uint8)
+    b_scale = b_byte.to(torch.uint8)[:, None].repeat(1, k // BLOCK)
+    v = 1 + torch.randint(0, 2, (m, k), device="cuda", generator=gen).double() / 2
+    power = 127 - torch.arange(m, device="cuda") * 254 // (m - 1)
+    if kind == "fp16":
+        power = power.clamp(-15, 14)
+    a64 = v * power64(power)[:, None]
+    if kind == "fp8":
+        a, a_scale = v.float().to(FP8), (power + 127).to(torch.uint8)[:, None].repeat(1, k // BLOCK)
+    else:
+        a, a_scale = a64.to(KINDS[kind]), None
+        assert torch.equal(a.double(), a64)
+    ones = torch.full_like(b_scale, 127)
+    return a, a_scale, a64, b, b_scale, from4(b, ones) * power64(b_byte - 127)[:, None]
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", [(12, 255, 160), (60, 509, 96), (255, 300, 160), (400, 33000, 160)])
+def test_every_scale_byte(m, n, k, kind):
+    """Scales from 2^-127 to 2^127 on either side. Values from 1 to 6 leave every sum
+    exact, and no two of its products are far apart."""
+    import flashinfer_amd as fi
+
+    a, a_scale, a64, b, b_scale, w64 = scale_operands(m, n, k, kind)
+    want = (a64 @ w64.T).to(torch.bfloat16)
+    out = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale, out_dtype=torch.bfloat16)
+    # results below the least normal number apart
+    seen = want.abs() >= 2.0 ** -126
+    assert seen.float().mean() > 0.4 and torch.equal(out[seen], want[seen])
+    assert (out[~seen].abs() <= 2.0 ** -126).all()
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m, n, k", [(12, 256, 160), (60, 512, 96), (255, 320, 160), (400, 16512, 160)])
+def test_every_scale_byte_and_mxfp8_outputs(m, n, k, kind):
+    import flashinfer_amd as fi
+
+    a, a_scale, a64, b, b_scale, w64 = scale_operands(m, n, k, kind)
+    b, b_scale, w64 = torch.cat((b, b)), torch.cat((b_scale, b_scale)), torch.cat((w64, w64))
+    g = a64 @ w64[:n].T
+    # silu(g) is g in 32 bits from about 20 on
+    y = (g * g).float()
+    plain = ((g > 20) & y.isfinite()).unflatten(1, (-1, BLOCK)).all(-1)
+    assert plain.float().mean() > 0.02
+    want_q, want_s = to8_bits(y)
+    q, s = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=FP8)
+    assert torch.equal(s[plain], want_s[plain])
+    q, want_q = (t.view(torch.uint8).unflatten(1, (-1, BLOCK)) for t in (q, want_q))
+    assert torch.equal(q[plain], want_q[plain])
+
+
+@gpu
+@pytest.mark.parametrize("kind", ["bf16", "fp16", "fp8"])
+@pytest.mark.parametrize("m", [4, 40, 100, 300])
+def test_weights_of_2_to_the_128(m, kind):
+    """What 16 bits do not hold is not finite, and nothing beside it is touched;
+    MXFP8 tokens take the scale as it is."""
+    import flashinfer_amd as fi
+
+    n, k = 64, 64
+    b = torch.zeros(n, k // 2, dtype=torch.uint8, device="cuda")
+    b_scale = torch.full((n, k // BLOCK), 127, dtype=torch.uint8, device="cuda")
+    b[:, 0] = 7
+    b[3, 0], b[4, 0], b[5, 0] = 6, 5, 3  # 4, 3 and 1.5
+    b_scale[:6, 0] = torch.tensor([252, 253, 254, 253, 253, 254], device="cuda")
+    a, a_scale = torch.full((m, k), 2.0 ** -14, device="cuda"), None
+    if kind == "fp8":
+        a, a_scale = fi.mxfp8_quantize(a)
+    else:
+        a = a.to(KINDS[kind])
+    level = torch.tensor([6, 6, 6, 4, 3, 1.5] + [6] * 58, device="cuda", dtype=torch.float64)
+    want = (level * power64(b_scale[:, 0].long() - 127) * 2.0 ** -14).to(torch.bfloat16)
+    out = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale, out_dtype=torch.bfloat16)
+    past = torch.zeros(n, dtype=torch.bool, device="cuda")
+    past[1:4] = kind != "fp8"
+    assert torch.equal(out[:, ~past], want[~past].expand(m, -1))
+    assert not out[:, past].isfinite().any()
