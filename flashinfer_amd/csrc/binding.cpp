@@ -951,10 +951,10 @@ bool on_16(const at::Tensor& t) {
 }
 
 // (out, out_scale) of x, of rmsnorm(x) * w, or of rmsnorm(residual += x) * w.
-std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tensor> residual,
-                                            c10::optional<at::Tensor> w,
-                                            c10::optional<at::Tensor> out,
-                                            c10::optional<at::Tensor> out_scale,
+std::tuple<at::Tensor, at::Tensor> mx_quant(const at::Tensor& x, const at::Tensor* residual,
+                                            const at::Tensor* w,
+                                            const c10::optional<at::Tensor>& out,
+                                            const c10::optional<at::Tensor>& out_scale,
                                             double eps) {
   const char* name = "MXFP8 output";
   TORCH_CHECK_VALUE(x.dim() >= 1, name, ": the input needs a last dimension");
@@ -1002,25 +1002,23 @@ std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tens
                       name, ": out_scale must be contiguous uint8 ", scale_shape, ", got ",
                       out_scale->scalar_type(), " ", out_scale->sizes());
   TORCH_CHECK_VALUE(x.is_cuda(), name, ": the input must be on a GPU, got ", x.device());
-  for (const auto* t : {&residual, &w, &out, &out_scale})
-    TORCH_CHECK_VALUE(!t->has_value() || (*t)->device() == x.device(), name,
-                      ": operands are on ", x.device(), " and ", (*t)->device());
-  const at::Tensor* r = residual ? &*residual : nullptr;
-  const at::Tensor* wp = w ? &*w : nullptr;
-  if (r) refuse_overlap(name, *r, {&x, wp});
-  if (out) refuse_overlap(name, *out, {&x, r, wp});
-  if (out_scale) refuse_overlap(name, *out_scale, {&x, r, wp, out ? &*out : nullptr});
+  for (const at::Tensor* t : {residual, w, out ? &*out : nullptr, out_scale ? &*out_scale : nullptr})
+    TORCH_CHECK_VALUE(!t || t->device() == x.device(), name, ": operands are on ", x.device(),
+                      " and ", t->device());
+  if (residual) refuse_overlap(name, *residual, {&x, w});
+  if (out) refuse_overlap(name, *out, {&x, residual, w});
+  if (out_scale) refuse_overlap(name, *out_scale, {&x, residual, w, out ? &*out : nullptr});
 
   c10::DeviceGuard guard(x.device());
   at::Tensor q = out ? *out : empty_like_on(x, x.sizes(), at::kFloat8_e4m3fn);
   at::Tensor s = out_scale ? *out_scale : empty_like_on(x, scale_shape, at::kByte);
   const int64_t step = 16 / x.element_size();
   const bool aligned = on_16(x) && (rows <= 1 || sx % step == 0) &&
-                       (!r || (on_16(*r) && (rows <= 1 || sr % step == 0))) &&
-                       (!wp || on_16(*wp)) &&
+                       (!residual || (on_16(*residual) && (rows <= 1 || sr % step == 0))) &&
+                       (!w || on_16(*w)) &&
                        reinterpret_cast<uintptr_t>(q.data_ptr()) % 8 == 0;
-  check_hip(fi_mx_quant(dtype_code(x), x.data_ptr(), r ? r->data_ptr() : nullptr,
-                        wp ? wp->data_ptr() : nullptr, q.data_ptr(), s.data_ptr(), (int)rows,
+  check_hip(fi_mx_quant(dtype_code(x), x.data_ptr(), residual ? residual->data_ptr() : nullptr,
+                        w ? w->data_ptr() : nullptr, q.data_ptr(), s.data_ptr(), (int)rows,
                         (int)K, sx, sr, eps, aligned, cur_stream(x)),
             "fi_mx_quant");
   return {q, s};
@@ -1028,20 +1026,24 @@ std::tuple<at::Tensor, at::Tensor> mx_quant(at::Tensor x, c10::optional<at::Tens
 
 // The three entries name what each of them needs: without its weight or its
 // residual a call is refused by its signature rather than computed as another one.
-std::tuple<at::Tensor, at::Tensor> mxfp8_quantize(at::Tensor x, c10::optional<at::Tensor> out,
-                                                  c10::optional<at::Tensor> out_scale) {
-  return mx_quant(x, c10::nullopt, c10::nullopt, out, out_scale, 0.0);
+std::tuple<at::Tensor, at::Tensor> mxfp8_quantize(const at::Tensor& x,
+                                                  const c10::optional<at::Tensor>& out,
+                                                  const c10::optional<at::Tensor>& out_scale) {
+  return mx_quant(x, nullptr, nullptr, out, out_scale, 0.0);
 }
-std::tuple<at::Tensor, at::Tensor> mxfp8_rmsnorm(at::Tensor x, at::Tensor w,
-                                                 c10::optional<at::Tensor> out,
-                                                 c10::optional<at::Tensor> out_scale, double eps) {
-  return mx_quant(x, c10::nullopt, w, out, out_scale, eps);
+std::tuple<at::Tensor, at::Tensor> mxfp8_rmsnorm(const at::Tensor& x, const at::Tensor& w,
+                                                 const c10::optional<at::Tensor>& out,
+                                                 const c10::optional<at::Tensor>& out_scale,
+                                                 double eps) {
+  return mx_quant(x, nullptr, &w, out, out_scale, eps);
 }
-std::tuple<at::Tensor, at::Tensor> mxfp8_add_rmsnorm(at::Tensor x, at::Tensor residual,
-                                                     at::Tensor w, c10::optional<at::Tensor> out,
-                                                     c10::optional<at::Tensor> out_scale,
+std::tuple<at::Tensor, at::Tensor> mxfp8_add_rmsnorm(const at::Tensor& x,
+                                                     const at::Tensor& residual,
+                                                     const at::Tensor& w,
+                                                     const c10::optional<at::Tensor>& out,
+                                                     const c10::optional<at::Tensor>& out_scale,
                                                      double eps) {
-  return mx_quant(x, residual, w, out, out_scale, eps);
+  return mx_quant(x, &residual, &w, out, out_scale, eps);
 }
 
 int mx_type(at::ScalarType t) {
