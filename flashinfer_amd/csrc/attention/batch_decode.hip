@@ -10,6 +10,11 @@
 //     ~30%) at its 2-wave occupancy, so ~3 iterations stay in flight.
 //   * QK dots use packed v_dot2_f32_bf16 (keeps K in bf16 registers, halves
 //     the VALU op count of the convert+FMA form).
+//   * A dot is summed over its token's lanes in registers, and the exponential is
+//     the instruction alone: through shared memory, and with a range reduction
+//     for results below 2^-126, their latency was the bound at two waves a SIMD
+//     once FP32 math came unpacked (256 requests of 32768, GQA 4: 7.13 -> 5.99 ms,
+//     4.82 -> 5.73 TB/s; 128 of 8192 925 -> 806 us).
 //   * GQA group (1/2/4/8 q heads per kv head) processed in-register against
 //     one K read — the K/V bytes are the bound, q reuse is free.
 //   * split-KV via host-planned work items (req, chunk); partials are written
@@ -192,9 +197,7 @@ __global__ __launch_bounds__(
           for (int j = 0; j < VPL; ++j) s += qv.get(j) * kv_cur.get(j);
         }
       }
-      // reduce across the LPT lanes of this token
-#pragma unroll
-      for (int off2 = LPT / 2; off2 > 0; off2 >>= 1) s += __shfl_xor(s, off2, 64);
+      s = lane_group_sum<LPT>(s);  // across the lanes of this token
       float s2;
       if constexpr (SOFT_CAP) {
         s2 = p.logits_soft_cap * tanhf(s * scale / p.logits_soft_cap) *
@@ -212,12 +215,12 @@ __global__ __launch_bounds__(
       }
       if (valid) {
         if (s2 <= m_run[g]) {
-          float pv = __builtin_exp2f(s2 - m_run[g]);
+          float pv = __builtin_amdgcn_exp2f(s2 - m_run[g]);
           d_run[g] += pv;
 #pragma unroll
           for (int j = 0; j < VPL; ++j) o_acc[g][j] += pv * vf[j];
         } else {
-          float r = __builtin_exp2f(m_run[g] - s2);  // exp2(-inf)=0 first time
+          float r = __builtin_amdgcn_exp2f(m_run[g] - s2);  // exp2(-inf)=0 first time
           d_run[g] = d_run[g] * r + 1.f;
 #pragma unroll
           for (int j = 0; j < VPL; ++j) o_acc[g][j] = __builtin_fmaf(o_acc[g][j], r, vf[j]);

@@ -47,6 +47,35 @@ __device__ __forceinline__ float xhalf_sum(float x) {
                                             __float_as_int(x), false, false);
   return __int_as_float(r[0]) + __int_as_float(r[1]);
 }
+
+// __shfl_xor(x, kOff, 64) for kOff of 1, 2, 4 and 8 in registers (a move across
+// lanes within a row of 16) where __shfl_xor waits for shared memory's way. All
+// lanes of the row must be active.
+template <int kOff>
+__device__ __forceinline__ float xor_lanes(float x) {
+  static_assert(kOff == 1 || kOff == 2 || kOff == 4 || kOff == 8, "");
+  const int v = __float_as_int(x);
+  if constexpr (kOff == 4) {
+    // lanes 0-3 and 8-11 take the lane 4 above, the others the lane 4 below
+    const int up = __builtin_amdgcn_update_dpp(0, v, 0x104, 0xf, 0x5, false);
+    return __int_as_float(__builtin_amdgcn_update_dpp(up, v, 0x114, 0xf, 0xA, false));
+  } else {
+    constexpr int kControl = kOff == 1 ? 0xB1 : kOff == 2 ? 0x4E : 0x128;
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, v, kControl, 0xf, 0xf, true));
+  }
+}
+
+// Sum over groups of kLanes lanes (16 at most in registers), the far halves first.
+template <int kLanes>
+__device__ __forceinline__ float lane_group_sum(float x) {
+  if constexpr (kLanes >= 64) x += __shfl_xor(x, 32, 64);
+  if constexpr (kLanes >= 32) x += __shfl_xor(x, 16, 64);
+  if constexpr (kLanes >= 16) x += xor_lanes<8>(x);
+  if constexpr (kLanes >= 8) x += xor_lanes<4>(x);
+  if constexpr (kLanes >= 4) x += xor_lanes<2>(x);
+  if constexpr (kLanes >= 2) x += xor_lanes<1>(x);
+  return x;
+}
 using fp8_e5m2 = __hip_fp8_e5m2;
 
 // Ext-vector typedefs (register-resident fragments and vector loads).
