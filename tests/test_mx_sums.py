@@ -204,3 +204,28 @@ def test_weights_of_2_to_the_128(m, kind):
     past[1:4] = kind != "fp8"
     assert torch.equal(out[:, ~past], want[~past].expand(m, -1))
     assert not out[:, past].isfinite().any()
+
+
+@gpu
+def test_norms_of_one_dimension_and_of_more_rows_than_a_launch():
+    """A row alone, and 2^21 rows and some, which go in two launches, inside wider
+    tensors: input, residual and outputs advance by their own strides."""
+    import flashinfer_amd as fi
+
+    k, rows = 64, 2 ** 21 + 5
+    w = torch.linspace(0.5, 2, k, device="cuda").bfloat16()
+    wide = torch.randn(7, 3 * k, device="cuda").bfloat16().repeat(rows // 7 + 1, 1)[:rows]
+    x, r = wide[:, :k], wide[:, k + 8:2 * k + 8]
+    few_x, few_r = x[:7].clone(), r[:7].clone()
+    beside = wide[:, 2 * k + 8:].clone()
+    want_q, want_s = fi.fused_add_rmsnorm_mxfp8_quant(few_x, few_r, w)
+    q, s = fi.fused_add_rmsnorm_mxfp8_quant(x, r, w)
+    for i in range(7):
+        assert bool((q[i::7].view(torch.uint8) == want_q[i].view(torch.uint8)).all())
+        assert bool((s[i::7] == want_s[i]).all()) and bool((r[i::7] == few_r[i]).all())
+    assert torch.equal(wide[:, 2 * k + 8:], beside)
+    for f in (fi.mxfp8_quantize, lambda t: fi.rmsnorm_mxfp8_quant(t, w)):
+        (q, s), (want_q, want_s) = f(few_x[2]), f(few_x)
+        assert q.shape == (k,) and s.shape == (k // BLOCK,)
+        assert torch.equal(q.view(torch.uint8), want_q[2].view(torch.uint8))
+        assert torch.equal(s, want_s[2])

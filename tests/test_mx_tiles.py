@@ -196,3 +196,18 @@ def test_more_tiles_than_one_launch():
         assert not q[at:at + 10000, :-32].view(torch.uint8).any()
     del q, s
     torch.cuda.empty_cache()
+
+
+@gpu
+@pytest.mark.parametrize("m", [3, 40, 300])
+def test_scales_as_float8_e8m0fnu(m):
+    import flashinfer_amd as fi
+
+    a, a_scale, _ = activations(m, 160, "fp8")
+    b, b_scale = weights4(192, 160)
+    e8m0 = torch.float8_e8m0fnu
+    want = fi.gemm_mxfp4_nt(a, b, b_scale, a_scale)
+    assert torch.equal(fi.gemm_mxfp4_nt(a, b, b_scale.view(e8m0), a_scale.view(e8m0)), want)
+    want_q, want_s = fi.gemm_mxfp4_nt_gated(a, b, b_scale, a_scale, out_dtype=FP8)
+    q, s = fi.gemm_mxfp4_nt_gated(a, b, b_scale.view(e8m0), a_scale.view(e8m0), out_dtype=FP8)
+    assert torch.equal(s, want_s) and torch.equal(q.view(torch.uint8), want_q.view(torch.uint8))
